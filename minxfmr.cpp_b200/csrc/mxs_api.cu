@@ -377,6 +377,16 @@ int sample_impl(const float* d_logits, int64_t rows, int64_t vocab, int64_t ld, 
 }  // namespace
 
 namespace mxs {
+int device_info(int* sms, uint32_t** status) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    Device* d;
+    int rc = current_device(&d);
+    if (rc) return rc;
+    *sms = d->sms;
+    *status = d->status;
+    return MXS_OK;
+}
+
 // Bytes at the start of every workspace layout on the current device that must
 // read zero when a call starts: the CTA-synchronous kernel's per-row chunk
 // counters, which sit at offsets that depend on the device alone. (The

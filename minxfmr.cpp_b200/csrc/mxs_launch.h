@@ -10,6 +10,8 @@ size_t sample_kernel_smem_bytes();
 cudaError_t sample_kernel_configure(int* blocks_per_sm);
 cudaError_t sample_kernel_launch(const Params& p, int grid, bool tma, cudaStream_t stream);
 int workspace_zero_prefix(size_t* bytes);  // mxs_api.cu
+// SM count and status word of the current device (MXS_OK, or the error current_device gives); mxs_api.cu
+int device_info(int* sms, uint32_t** status);
 
 // The row lists a vocab-sharded shard step leaves in the library workspace
 // (two-kernel path only): every logit of a chunk's later tiles above a

@@ -3,7 +3,7 @@
 Only sm_100a code is generated. Each translation unit compiles to its own
 object (in parallel, rebuilt only when it or a header is newer); the library
 links the CUDA runtime statically and exports exactly the functions of
-include/mxs_sampler.h.
+include/mxs_sampler.h and include/mxs_head.h.
     python minxfmr.cpp_b200/mxs_build.py [--verbose] [--profile]
 """
 import os
@@ -17,7 +17,8 @@ OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libmxs.so")
 # phase-timer build (-DMXS_PROFILE) for kernel analysis; never loaded by the product path
 PROF_LIB = os.path.join(OUT_DIR, "libmxs_prof.so")
-SOURCES = ["mxs_sampler.cu", "mxs_stream.cu", "mxs_api.cu", "mxs_noalloc.cu", "mxs_multi.cu", "mxs_hidden.cu"]
+SOURCES = ["mxs_sampler.cu", "mxs_stream.cu", "mxs_api.cu", "mxs_noalloc.cu", "mxs_multi.cu", "mxs_hidden.cu",
+           "mxs_ce.cu", "mxs_fp8.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 COMPILE_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -41,7 +42,7 @@ def build(verbose=False, force=False, profile=False):
     obj_dir = os.path.join(OUT_DIR, "obj_prof" if profile else "obj")
     os.makedirs(obj_dir, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cu")] + [
-        os.path.join(HERE, "..", "include", "mxs_sampler.h")]
+        os.path.join(HERE, "..", "include", f) for f in ("mxs_sampler.h", "mxs_head.h")]
     newest_header = max(os.path.getmtime(h) for h in headers)
     extra = (["-Xptxas", "-v"] if verbose else []) + (["-DMXS_PROFILE"] if profile else [])
 

@@ -1,5 +1,6 @@
 """Python host side of the B200 token sampler: ctypes bindings over the C ABI
-(include/mxs_sampler.h, built into minxfmr.cpp_b200/lib/libmxs.so).
+(include/mxs_sampler.h and include/mxs_head.h, built into
+minxfmr.cpp_b200/lib/libmxs.so).
 
 The sampler is the drop-in for the sampling block of the reference's
 minxfmr_generate (src/api/minxfmr.cpp:2091-2171). `sample()` mirrors that
@@ -35,13 +36,16 @@ ROW_TIMEOUT = 8
 TOKEN_NOT_FIRST = 1
 TOKEN_EOS = 2
 
-# Every symbol include/mxs_sampler.h declares.
+# Every symbol include/mxs_sampler.h and include/mxs_head.h declare.
 EXPORTS = (
     "mxs_sample_topk", "mxs_sample_topk_ex", "mxs_workspace_size", "mxs_workspace_init",
     "mxs_sample_topk_host", "mxs_shard_candidates", "mxs_merge_sample", "mxs_get_status",
     "mxs_version", "mxs_sample_topk_noalloc", "mxs_set_profile_events", "mxs_sample_rowsharded",
     "mxs_sample_vocabsharded", "mxs_set_test_hooks", "mxs_vocabsharded_stats", "mxs_sample_topk_edits",
     "mxs_token_checks", "mxs_sample_from_hidden",
+    "mxs_ce_from_hidden", "mxs_ce_from_hidden_backward", "mxs_ce_workspace_size", "mxs_quantize_fp8",
+    "mxs_matmul_fp8", "mxs_matmul_fp8_workspace_size", "mxs_sample_from_hidden_fp8",
+    "mxs_sample_from_hidden_fp8_workspace_size",
 )
 
 _P = ctypes.c_void_p
@@ -70,6 +74,16 @@ _SIGS = {
     "mxs_sample_from_hidden": [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _I, _D, _D, _P, _P, _P, _P, _P, _I64, _P],
     "mxs_sample_topk_edits": [_P, _I64, _I64, _I64, _D, _I, _D, _D, _P, _I, _P, _I64, _P, _I, _D, _D, _D, _P, _P,
                               _P, _P, _P, _P],
+    "mxs_ce_from_hidden": [_P, _I64, _P, _I64, _I, _I64, _I64, _I64, _P, _I, _D, _P, _P, _P, _SZ, _P],
+    "mxs_ce_from_hidden_backward": [_P, _I64, _P, _I64, _I, _I64, _I64, _I64, _P, _I, _D, _P, _P, _P, _I64, _P, _I64,
+                                    _P, _SZ, _P],
+    "mxs_ce_workspace_size": [_P, _I64, _I64, _I64, _I64, _I, ctypes.POINTER(_SZ)],
+    "mxs_quantize_fp8": [_P, _I64, _I, _I64, _I64, _I, _P, _I64, _P, _P],
+    "mxs_matmul_fp8": [_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I, _P, _SZ, _P],
+    "mxs_matmul_fp8_workspace_size": [_P, _I64, _P, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "mxs_sample_from_hidden_fp8": [_P, _I64, _I, _P, _I64, _P, _I64, _I64, _I64, _D, _I, _D, _D, _P, _P, _P, _P, _P,
+                                   _I64, _P, _SZ, _P],
+    "mxs_sample_from_hidden_fp8_workspace_size": [_P, _I64, _I64, _I64, _I64, _I, ctypes.POINTER(_SZ)],
 }
 
 _lib = None
@@ -435,3 +449,7 @@ def get_status(clear=True):
 
 def version():
     return load().mxs_version().decode()
+
+
+from .head import (ce_from_hidden, ce_from_hidden_backward, cross_entropy_from_hidden, matmul_fp8,  # noqa: E402
+                   quantize_fp8, sample_from_hidden_fp8)
