@@ -386,6 +386,7 @@ int device_info(int* sms, uint32_t** status) {
     *status = d->status;
     return MXS_OK;
 }
+int64_t test_drop_tile() { return g_hooks.drop_tile; }
 
 // Bytes at the start of every workspace layout on the current device that must
 // read zero when a call starts: the CTA-synchronous kernel's per-row chunk

@@ -22,7 +22,9 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
+#include "mxs_gemm.cuh"
 #include "mxs_head.cuh"
 #include "mxs_launch.h"
 
@@ -31,8 +33,10 @@ namespace {
 using mxs::Carve;
 using mxs::ceil_div;
 using mxs::round_up;
-using mxs::to_f32;
+using mxs::gemm::Ctx;
+using mxs::gemm::Tile;
 
+constexpr int64_t MAX_DIM = INT32_MAX - 1024;
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.4426950408889634074;
 
@@ -40,6 +44,14 @@ struct Head {
     int kept;      // rows with a target in range
     float gmax;    // largest finite |grad_loss| of those rows (1 if none)
 };
+
+// Splits of K for `tiles` grad_hidden tiles: as many as fill the units, at least
+// 8 blocks of 64 columns each. A fixed function of the shape: the same sums in the same order every time.
+__host__ __device__ inline int grad_hidden_splits(int tiles, int width, int units) {
+    const int most = (width + 511) / 512;
+    const int s = tiles > 0 ? units / tiles : 1;
+    return s < 1 ? 1 : s < most ? s : most;
+}
 
 struct Pack {
     const void* hidden;
@@ -74,9 +86,9 @@ constexpr int PACK_TAIL = 256;  // rows after the last kept one that read zero
 // range itself (a few KB of targets from L2), so one launch does it all.
 template <typename T>
 __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
+    mxs::gemm::grid_launch_dependents();
     __shared__ int s_cnt[PACK_T / 32];
     __shared__ float s_max[PACK_T / 32];
-    __shared__ int s_base;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (int)ceil_div(p.rows, gridDim.x);
     const int r0 = min(p.rows, (int)blockIdx.x * per), r1 = min(p.rows, r0 + per);
@@ -158,85 +170,108 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
         for (int64_t i = tid; i < (int64_t)(end - base) * p.ldk; i += PACK_T)
             static_cast<T*>(p.packed)[(int64_t)base * p.ldk + i] = mxs::from_f32<T>(0.0f);
     }
-    (void)s_base;
 }
 
 // ---------------------------------------------------------------------------
-// Products: 64 x 64 tiles in fp32 through shared memory.
+// Logit tiles (forward): rows of H against rows of W, both K-major.
 // ---------------------------------------------------------------------------
-constexpr int TM = 64, TN = 64, TK = 16;
 
-template <typename LA, typename LB>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], int K, LA la, LB lb) {
-    __shared__ float sa[TK][TM + 4], sb[TK][TN + 4];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    for (int k0 = 0; k0 < K; k0 += TK) {
-        __syncthreads();
-        for (int i = tid; i < TM * TK; i += 256) {
-            const int k = i % TK, m = i / TK;
-            sa[k][m] = k0 + k < K ? la(m, k0 + k) : 0.0f;
-            sb[k][m] = k0 + k < K ? lb(m, k0 + k) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
-    }
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2^-22 relative; results below 2^-126 are 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-struct Score {
-    const void* h;   // packed rows
-    const void* w;
-    int64_t ldw;
-    int d, ldk, vocab;
-    float c;         // log2(e) / temperature
+// What the two passes over the logits share: the tiles' walk (rows fastest, so
+// the tiles in flight share their weight rows in L2) and the loads.
+template <int CG_>
+struct LogitTiles {
+    static constexpr int CG = CG_;
+    static constexpr bool F8 = false, PROMOTE = false;
+    CUtensorMap mh, mw;
+    int format;
+    int64_t drop;
+    uint32_t* status;
     const Head* head;
     const int* target;
-    float2* part;    // [tile][rows]: largest y of the others, sum 2^(y - largest)
-    float* ytarget;  // [rows]
-    int rows;
+    int rows, vocab;     // vocab: columns of this pass (its piece), starting at v0
+    int v0, n, nt, kblocks, a_rows;
+    float c;             // log2(e) / temperature
+
+    __device__ void prefetch() const {
+        mxs::gemm::prefetch_map(&mh);
+        mxs::gemm::prefetch_map(&mw);
+    }
+    __device__ int kept() const { return *(volatile const int*)&head->kept; }
+    __device__ bool tile(int i, const Ctx& x, Tile& t) const {
+        const int mt = (x.kept + 128 * CG - 1) / (128 * CG);
+        const int64_t idx = x.unit + (int64_t)i * x.units;
+        if (idx >= (int64_t)mt * nt) return false;
+        const int m = (int)(idx % mt), v = (int)(idx / mt);
+        t = Tile{m * 128 * CG, v * n, 0, kblocks, n, v};
+        return true;
+    }
+    __device__ bool a_mn(const Tile&) const { return false; }
+    __device__ bool b_mn(const Tile&) const { return false; }
+    __device__ uint32_t bytes(const Tile&) const { return (uint32_t)(a_rows + n / CG) * 128; }
+    __device__ void load(const Tile& t, int kb, uint32_t sa, uint32_t sb, uint32_t bar, const Ctx& x) const {
+        mxs::gemm::tma_load<CG>(sa, &mh, kb * 64, t.m0 + (int)x.rank * 128, bar);
+        mxs::gemm::tma_load<CG>(sb, &mw, kb * 64, v0 + t.n0 + (int)x.rank * (n / CG), bar);
+    }
+    __device__ void zero(const Tile&, int, int, const Ctx&) const {}
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) score_kernel(const Score p) {
-    const int kept = p.head->kept;
-    const int m0 = blockIdx.y * TM, v0 = blockIdx.x * TN;
-    if (m0 >= kept) return;
-    float acc[4][4] = {};
-    const T *h = static_cast<const T*>(p.h), *w = static_cast<const T*>(p.w);
-    tile_product(acc, p.d,
-                 [&](int m, int k) { return m0 + m < kept ? to_f32(h[(int64_t)(m0 + m) * p.ldk + k]) : 0.0f; },
-                 [&](int n, int k) { return v0 + n < p.vocab ? to_f32(w[(int64_t)(v0 + n) * p.ldw + k]) : 0.0f; });
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int i = 0; i < 4; ++i) {
-        const int r = m0 + ty * 4 + i;
-        const int t = r < kept ? p.target[r] : -1;
+// Each thread holds half a tile's columns of one row: the largest y of the others
+// and sum 2^(y - largest). The exponentials run at 16 a clock and SM: 2048 clocks
+// for 128 x 256, under the 512 clocks of each 64 of d_model that the products take.
+template <int CG_>
+struct ScoreOp : LogitTiles<CG_> {
+    float2* part;    // [tile * 2 + half][rows]
+    float* ytarget;  // [rows]
+
+    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
+        const int r = t.m0 + row;
+        if ((r & ~31) >= x.kept) return;  // no row of this warp
+        const int hit = r < x.kept ? this->target[r] - t.n0 : -1;  // the target's column of this tile
+        const int cols = min(t.n, this->vocab - t.n0);
         float m = -INFINITY, s = 0.0f;
-        for (int j = 0; j < 4; ++j) {
-            const int v = v0 + tx * 4 + j;
-            acc[i][j] *= p.c;
-            if (v == t) p.ytarget[r] = acc[i][j];
-            if (v < p.vocab && v != t) m = fmaxf(m, acc[i][j]);
+        for (int c0 = half * 32; c0 < t.n; c0 += 64) {
+            float v[32];
+            mxs::gemm::tmem_ld32(tmem + c0, v);
+            if (hit >= c0 && hit < c0 + 32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j == hit - c0) {
+                        ytarget[r] = v[j] * this->c;
+                        v[j] = -INFINITY;
+                    }
+            }
+            if (c0 + 32 > cols) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c0 + j >= cols) v[j] = -INFINITY;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+            const float nm = fmaxf(m, top * this->c);
+            const float sub = nm == -INFINITY ? 0.0f : nm;
+            float sum[4] = {s * ex2(m - sub), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[j & 3] += ex2(fmaf(v[j], this->c, -sub));
+            s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            m = nm;
         }
-        for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float sub = m == -INFINITY ? 0.0f : m;
-        for (int j = 0; j < 4; ++j) {
-            const int v = v0 + tx * 4 + j;
-            if (v < p.vocab && v != t) s += exp2f(acc[i][j] - sub);
-        }
-        for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (tx == 0 && r < kept) p.part[(int64_t)blockIdx.x * p.rows + r] = make_float2(m, s);
+        if (r < x.kept) part[((int64_t)t.kind * 2 + half) * this->rows + r] = make_float2(m, s);
     }
-}
+};
 
 // One warp per row joins the tiles' pairs, in the same order every time.
 __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, const float* ytarget, const int* pos,
                                                          int rows, int tiles, float* loss, float* lse) {
     const int lane = threadIdx.x & 31;
     const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+    mxs::gemm::grid_wait();
     if (r >= rows) return;
     const int at = pos[r];
     if (at < 0) {
@@ -269,97 +304,222 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, con
     }
 }
 
-struct Grad {
-    const void *h, *w;
-    int64_t ldw;
-    int d, ldk, vocab, v0, width, ldg;  // the piece [v0, v0 + width) of the vocabulary; G is [rows][ldg]
-    float c;
-    float inv_t;
-    const Head* head;
-    const int* target;
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half*) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 values to `out`, as 16-byte stores where `vec` says that they are aligned.
+template <typename T>
+__device__ __forceinline__ void store32(T* out, const float (&v)[32], int n, bool vec) {
+    if (vec && n >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            T* tag = nullptr;
+            *reinterpret_cast<uint4*>(out + j) =
+                make_uint4(pack2(v[j], v[j + 1], tag), pack2(v[j + 2], v[j + 3], tag), pack2(v[j + 4], v[j + 5], tag),
+                           pack2(v[j + 6], v[j + 7], tag));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < n) out[j] = mxs::from_f32<T>(v[j]);
+    }
+}
+
+// The logits of a piece again, left as G = ghat (softmax - hot) in the operands'
+// type (rounded once; the products that read it accumulate in fp32). Rows after
+// the last kept one and columns after the piece read zero.
+template <int CG_, typename T>
+struct GradLogitsOp : LogitTiles<CG_> {
     const float *lse2, *ghat;
-    void* g;
-    float* acc;  // [rows][d] sums of grad_hidden
-    bool first;
-    void* dw;
-    int64_t lddw;
-    float gscale, inv_gscale;  // G is held times gscale (a power of two)
+    T* g;
+    int ldg;
+    float gscale;
+
+    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
+        const int r = t.m0 + row;
+        const bool live = r < x.kept;
+        const bool any = (r & ~31) < x.kept;
+        const int hit = live ? this->target[r] - this->v0 - t.n0 : -1;
+        const float l2 = live ? lse2[r] : 0.0f;
+        const float gr = live ? ghat[r] * gscale : 0.0f;
+        const int cols = live ? this->vocab - t.n0 : 0;
+        T* out = g + (int64_t)r * ldg + t.n0;
+        for (int c0 = half * 32; c0 < t.n; c0 += 64) {
+            float v[32];
+            if (any) {
+                mxs::gemm::tmem_ld32(tmem + c0, v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->c, -l2)) * gr;
+                if (hit >= c0 && hit < c0 + 32) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j == hit - c0) v[j] -= gr;
+                }
+            }
+            if (!any || c0 + 32 > cols) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c0 + j >= cols) v[j] = 0.0f;
+            }
+            store32(out + c0, v, ldg - t.n0 - c0, true);
+        }
+    }
 };
 
+// Both products of a piece in one launch. kind 0: grad_hidden += G W (M rows, N
+// d_model, K the piece's columns, cut into `splits` where the tiles alone are
+// fewer than the pairs); kind 1: grad_weight = G^T H (M the piece's columns, N
+// d_model, K rows). G is read K-major for the first and M-major for the second.
 template <typename T>
-__global__ void __launch_bounds__(256) grad_logits_kernel(const Grad p) {
-    const int kept = p.head->kept;
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN;
-    if (m0 >= kept) return;
-    float acc[4][4] = {};
-    const T *h = static_cast<const T*>(p.h), *w = static_cast<const T*>(p.w) + (int64_t)p.v0 * p.ldw;
-    tile_product(acc, p.d,
-                 [&](int m, int k) { return m0 + m < kept ? to_f32(h[(int64_t)(m0 + m) * p.ldk + k]) : 0.0f; },
-                 [&](int n, int k) { return n0 + n < p.width ? to_f32(w[(int64_t)(n0 + n) * p.ldw + k]) : 0.0f; });
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (r >= kept || n >= p.width) continue;
-            const float q = exp2f(fmaf(acc[i][j], p.c, -p.lse2[r])) - (p.v0 + n == p.target[r] ? 1.0f : 0.0f);
-            static_cast<T*>(p.g)[(int64_t)r * p.ldg + n] = mxs::from_f32<T>(q * (p.ghat[r] * p.gscale));
-        }
-}
+struct ProductOp {
+    static constexpr int CG = 2;
+    static constexpr bool F8 = false, PROMOTE = false;
+    CUtensorMap g_k, g_m, w_n, h_n;
+    int format;
+    int64_t drop;
+    uint32_t* status;
+    const Head* head;
+    int v0, width, d, n, nt;  // nt tiles of n columns over d
+    int split_width;          // the widest piece: what the number of splits goes by
+    float* acc;               // sums of grad_hidden, a block of 256 x 256 per tile and split
+    bool first, want_h, want_w;
+    T* dw;
+    int64_t lddw;
+    float scale;              // 1 / temperature / (G's own power of two)
+    bool vec;
 
-template <typename T>
-__global__ void __launch_bounds__(256) grad_hidden_kernel(const Grad p) {
-    const int kept = p.head->kept;
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN;
-    if (m0 >= kept) return;
-    float acc[4][4] = {};
-    const T *g = static_cast<const T*>(p.g), *w = static_cast<const T*>(p.w) + (int64_t)p.v0 * p.ldw;
-    tile_product(acc, p.width,
-                 [&](int m, int k) { return m0 + m < kept ? to_f32(g[(int64_t)(m0 + m) * p.ldg + k]) : 0.0f; },
-                 [&](int n, int k) { return n0 + n < p.d ? to_f32(w[(int64_t)k * p.ldw + n0 + n]) : 0.0f; });
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (r >= kept || n >= p.d) continue;
-            float* a = p.acc + (int64_t)r * p.d + n;
-            *a = p.first ? acc[i][j] : *a + acc[i][j];
+    __device__ void prefetch() const {
+        mxs::gemm::prefetch_map(&g_k);
+        mxs::gemm::prefetch_map(&g_m);
+        mxs::gemm::prefetch_map(&w_n);
+        mxs::gemm::prefetch_map(&h_n);
+    }
+    __device__ int kept() const { return *(volatile const int*)&head->kept; }
+    // The grad_hidden tiles go round the pairs first; when they leave some pairs
+    // with one tile fewer, those take the grad_weight tiles of the same cost before the rest go round.
+    __device__ bool tile(int i, const Ctx& x, Tile& t) const {
+        const int mh = want_h ? (x.kept + 255) / 256 : 0, th = mh * nt;
+        const int splits = grad_hidden_splits(th, split_width, x.units);
+        const int kh = (width + 63) / 64, kw = (x.kept + 63) / 64;
+        const int nh = th * splits;
+        const int mine = (nh - x.unit + x.units - 1) / x.units;  // grad_hidden tiles of this unit
+        if (i < mine) {
+            const int idx = x.unit + i * x.units;
+            const int tileno = idx % th, s = idx / th;
+            const int per = (kh + splits - 1) / splits;
+            const int k0 = min(kh, s * per);
+            t = Tile{tileno / nt * 256, tileno % nt * n, k0, min(kh, k0 + per) - k0, n, tileno * splits + s};
+            return true;
         }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) grad_weight_kernel(const Grad p) {
-    const int kept = p.head->kept;
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN;
-    float acc[4][4] = {};
-    const T *g = static_cast<const T*>(p.g), *h = static_cast<const T*>(p.h);
-    tile_product(acc, kept,
-                 [&](int m, int k) { return m0 + m < p.width ? to_f32(g[(int64_t)k * p.ldg + m0 + m]) : 0.0f; },
-                 [&](int n, int k) { return n0 + n < p.d ? to_f32(h[(int64_t)k * p.ldk + n0 + n]) : 0.0f; });
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float s = p.head->gmax * p.inv_t * p.inv_gscale;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= p.width || n >= p.d) continue;
-            static_cast<T*>(p.dw)[(int64_t)(p.v0 + m) * p.lddw + n] = mxs::from_f32<T>(acc[i][j] * s);
+        if (!want_w) return false;
+        const int64_t total = (int64_t)((width + 255) / 256) * nt;
+        const int over = nh % x.units;  // units [0, over) have one tile more
+        const int ahead = over == 0 || kw == 0 ? 0 : ((kh + splits - 1) / splits + kw / 2) / kw;
+        int j = i - mine;
+        int64_t idx;
+        if (x.unit >= over && j < ahead) {
+            idx = x.unit - over + (int64_t)j * (x.units - over);
+        } else {
+            if (x.unit >= over) j -= ahead;
+            idx = (int64_t)ahead * (x.units - over) + x.unit + (int64_t)j * x.units;
         }
-}
+        if (idx >= total) return false;
+        t = Tile{(int)(idx / nt) * 256, (int)(idx % nt) * n, 0, kw, n, -1};
+        return true;
+    }
+    __device__ bool a_mn(const Tile& t) const { return t.kind < 0; }
+    __device__ bool b_mn(const Tile&) const { return true; }
+    __device__ uint32_t bytes(const Tile&) const { return (uint32_t)(128 + n / 2) * 128; }
+    __device__ void load(const Tile& t, int kb, uint32_t sa, uint32_t sb, uint32_t bar, const Ctx& x) const {
+        const int m = t.m0 + (int)x.rank * 128, c = t.n0 + (int)x.rank * (n / 2), k = kb * 64;
+        if (t.kind >= 0) {
+            mxs::gemm::tma_load<2>(sa, &g_k, k, m, bar);
+        } else {
+            mxs::gemm::tma_load<2>(sa, &g_m, m, k, bar);
+            mxs::gemm::tma_load<2>(sa + 8192, &g_m, m + 64, k, bar);
+        }
+        const CUtensorMap* b = t.kind >= 0 ? &w_n : &h_n;
+        const int kr = t.kind >= 0 ? v0 + k : k;
+        for (int j = 0; j < n / 128; ++j) mxs::gemm::tma_load<2>(sb + j * 8192, b, c + 64 * j, kr, bar);
+    }
+    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx&) const {
+        if (t.kind >= 0) {
+            float* a = acc + ((int64_t)t.kind * 256 + row) * 256;
+            for (int c0 = half * 32; c0 < n; c0 += 64) {
+                float v[32];
+                mxs::gemm::tmem_ld32(tmem + c0, v);
+                float4* p = reinterpret_cast<float4*>(a + c0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float4 q = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    if (!first) {
+                        const float4 o = p[j];
+                        q = make_float4(q.x + o.x, q.y + o.y, q.z + o.z, q.w + o.w);
+                    }
+                    p[j] = q;
+                }
+            }
+            return;
+        }
+        const float s = head->gmax * scale;
+        const int m = t.m0 + row;
+        T* out = dw + (int64_t)(v0 + m) * lddw + t.n0;
+        for (int c0 = half * 32; c0 < n; c0 += 64) {
+            float v[32];
+            mxs::gemm::tmem_ld32(tmem + c0, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= s;
+            if (m < width) store32(out + c0, v, d - t.n0 - c0, vec);
+        }
+    }
+    __device__ void zero(const Tile& t, int row, int half, const Ctx&) const {
+        if (t.kind >= 0) {  // a split without columns
+            float* a = acc + ((int64_t)t.kind * 256 + row) * 256;
+            if (first)
+                for (int c0 = half * 128; c0 < min(n, half * 128 + 128); ++c0) a[c0] = 0.0f;
+            return;
+        }
+        const int m = t.m0 + row;
+        if (m >= width) return;
+        T* out = dw + (int64_t)(v0 + m) * lddw + t.n0;
+        for (int c0 = half * 128; c0 < min(min(n, half * 128 + 128), d - t.n0); ++c0) out[c0] = mxs::from_f32<T>(0.0f);
+    }
+};
 
-// grad_hidden of every row from the packed sums (rows left out: zero).
+// grad_hidden of every row: its tiles' splits added in order, times the scale
+// (rows left out: zero).
 template <typename T>
 __global__ void __launch_bounds__(256) grad_hidden_out_kernel(const float* acc, const int* pos, const Head* head,
-                                                              int d, float scale, T* out, int64_t ld) {
+                                                              int d, int n, int width, int units, float scale, T* out,
+                                                              int64_t ld) {
+    mxs::gemm::grid_wait();
     const int64_t r = blockIdx.x;
     const int at = pos[r];
     const float s = head->gmax * scale;
-    for (int k = threadIdx.x; k < d; k += 256)
-        out[r * ld + k] = mxs::from_f32<T>(at < 0 ? 0.0f : acc[(int64_t)at * d + k] * s);
+    const int nt = (d + n - 1) / n, splits = grad_hidden_splits((head->kept + 255) / 256 * nt, width, units);
+    for (int k = threadIdx.x; k < d; k += 256) {
+        float v = 0.0f;
+        if (at >= 0) {
+            const int64_t tile = (int64_t)(at / 256) * nt + k / n;
+            const float* a = acc + (tile * splits * 256 + at % 256) * 256 + k % n;
+            for (int i = 0; i < splits; ++i) v += a[(int64_t)i * 65536];
+        }
+        out[r * ld + k] = mxs::from_f32<T>(at < 0 ? 0.0f : v * s);
+    }
 }
 
 // ---------------------------------------------------------------------------
 // Plan
 // ---------------------------------------------------------------------------
-constexpr int PIECE = 8192;  // columns of G held at a time
+// G is held for a piece of the vocabulary at a time: about this many bytes, so
+// that the two products that read it find it in L2.
+constexpr int64_t PIECE_BYTES = 64 << 20;
 
 struct Plan {
     Head* head;
@@ -368,28 +528,42 @@ struct Plan {
     float2* part;
     float *ytarget, *lse2, *ghat, *acc;
     void* g;
-    int ldk, ldg;
+    void* w;          // the weight in aligned rows, if its own are not
+    int ldk;
+    int n, nt;        // logit tiles
+    int dn, dnt;      // tiles over d_model
+    int64_t piece;
     size_t bytes;
 };
 
-Plan make_plan(void* ws, int64_t rows, int64_t d, int64_t vocab, bool backward) {
+Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows, int64_t d, int64_t vocab,
+               bool backward) {
     Plan pl{};
     Carve c(ws);
+    rows = std::max<int64_t>(rows, 1);
     const int64_t rp = round_up(rows, PACK_TAIL);
+    const int cg = rows > 128 ? 2 : 1;
     pl.ldk = (int)round_up(d, 8);
     pl.head = c.take<Head>(1);
     pl.packed = c.take<uint16_t>((size_t)rp * pl.ldk);
     pl.pos = c.take<int>(rows);
     pl.target = c.take<int>(rows);
+    pl.w = mxs::aligned16(weight, 2 * ldw) ? nullptr : c.take<uint16_t>((size_t)vocab * pl.ldk);
     if (!backward) {
-        pl.part = c.take<float2>((size_t)ceil_div(vocab, TN) * rows);
+        pl.n = mxs::tile_width(ceil_div(rows, 128 * cg), vocab, sms / cg, 64, 32);
+        pl.nt = (int)ceil_div(vocab, pl.n);
+        pl.part = c.take<float2>((size_t)pl.nt * 2 * rows);
         pl.ytarget = c.take<float>(rows);
     } else {
         pl.lse2 = c.take<float>(rows);
         pl.ghat = c.take<float>(rows);
-        pl.ldg = (int)std::min<int64_t>(PIECE, round_up(vocab, 64));
-        pl.g = c.take<uint16_t>((size_t)rp * pl.ldg);
-        pl.acc = c.take<float>((size_t)rp * d);
+        const int64_t most = std::max<int64_t>(256, PIECE_BYTES / (2 * rp));
+        pl.piece = round_up(ceil_div(vocab, ceil_div(vocab, most)), 256);
+        pl.n = mxs::tile_width(ceil_div(rows, 128 * cg), pl.piece, sms / cg, 64, 64);
+        pl.g = c.take<uint16_t>((size_t)rp * pl.piece);
+        pl.dn = d > 128 ? 256 : 128;
+        pl.dnt = (int)ceil_div(d, pl.dn);
+        pl.acc = c.take<float>((size_t)std::max<int64_t>(rp / 256 * pl.dnt, sms / 2) * 65536);
     }
     pl.bytes = c.used;
     return pl;
@@ -397,15 +571,172 @@ Plan make_plan(void* ws, int64_t rows, int64_t d, int64_t vocab, bool backward) 
 
 bool bad_shape(int64_t ld_hidden, int64_t ld_weight, int dtype, int64_t rows, int64_t d, int64_t vocab,
                int target_bytes, double temperature) {
-    return rows < 0 || d <= 0 || vocab <= 0 || rows > INT32_MAX - 256 || d > INT32_MAX - 256 ||
-           vocab > INT32_MAX - 256 || ld_hidden < d || ld_weight < d || (dtype != MXS_BF16 && dtype != MXS_F16) ||
-           (target_bytes != 4 && target_bytes != 8) || !(temperature > 0.0) || !std::isfinite(temperature);
+    return rows < 0 || d <= 0 || vocab <= 0 || rows > MAX_DIM || d > MAX_DIM || vocab > MAX_DIM || ld_hidden < d ||
+           ld_weight < d || (dtype != MXS_BF16 && dtype != MXS_F16) || (target_bytes != 4 && target_bytes != 8) ||
+           !(temperature > 0.0) || !std::isfinite(temperature);
 }
 
 template <typename T>
-int launch_pack(const Pack& p, int sms, cudaStream_t st) {
-    pack_rows_kernel<T><<<(int)std::min<int64_t>(p.rows, sms * 2), PACK_T, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+constexpr int format_of() { return std::is_same<T, __half>::value ? 0 : 1; }
+
+// A kernel that may start while the one before it drains.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*k)(P...), unsigned grid, unsigned block, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...);
+}
+
+struct Call {
+    const void* hidden;
+    int64_t ldh;
+    const void* weight;
+    int64_t ldw;
+    int64_t rows, d, vocab;
+    const void* targets;
+    int tb;
+    double temperature;
+    int sms;
+    uint32_t* status;
+    cudaStream_t st;
+};
+
+#define MXS_TRY(e)                               \
+    do {                                         \
+        if ((e) != cudaSuccess) return MXS_ERR_CUDA; \
+    } while (0)
+
+template <typename T>
+int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad) {
+    const Pack p{a.hidden, a.ldh, a.targets, a.tb, (int)a.rows, (int)a.d, pl.ldk, a.vocab, lse, grad,
+                 pl.head, pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat};
+    pack_rows_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, a.sms * 2), PACK_T, 0, a.st>>>(p);
+    MXS_TRY(cudaGetLastError());
+    return MXS_OK;
+}
+
+template <int CG, typename T>
+int logit_tiles(LogitTiles<CG>& op, const Call& a, const Plan& pl, const void* w, int64_t ldw) {
+    op.format = format_of<T>();
+    op.drop = mxs::test_drop_tile();
+    op.status = a.status;
+    op.head = pl.head;
+    op.target = pl.target;
+    op.rows = (int)a.rows;
+    op.n = pl.n;
+    op.kblocks = (int)ceil_div(a.d, 64);
+    op.a_rows = CG == 1 ? (int)round_up(a.rows, 8) : 128;
+    op.c = (float)(LOG2E / a.temperature);
+    // rows of the tile that the box leaves out keep what shared memory held: their results are not read
+    if (!mxs::gemm::make_map(&op.mh, pl.packed, 2, a.d, round_up(a.rows, PACK_TAIL), pl.ldk, op.a_rows) ||
+        !mxs::gemm::make_map(&op.mw, w, 2, a.d, a.vocab, ldw, pl.n / CG))
+        return MXS_ERR_CUDA;
+    return MXS_OK;
+}
+
+template <int CG, typename T>
+int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss, float* lse) {
+    ScoreOp<CG> op{};
+    int rc = logit_tiles<CG, T>(op, a, pl, w, ldw);
+    if (rc) return rc;
+    op.vocab = (int)a.vocab;
+    op.nt = pl.nt;
+    op.part = pl.part;
+    op.ytarget = pl.ytarget;
+    const int64_t tiles = ceil_div(a.rows, 128 * CG) * pl.nt;
+    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
+    MXS_TRY(launch_dependent(score_join_kernel, (unsigned)ceil_div(a.rows, 8), 256, a.st, pl.part, pl.ytarget, pl.pos,
+                             (int)a.rows, pl.nt * 2, loss, lse));
+    return MXS_OK;
+}
+
+template <int CG, typename T>
+int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_t v0, ProductOp<T>& prod) {
+    GradLogitsOp<CG, T> op{};
+    int rc = logit_tiles<CG, T>(op, a, pl, w, ldw);
+    if (rc) return rc;
+    op.v0 = (int)v0;
+    op.vocab = (int)std::min(pl.piece, a.vocab - v0);
+    op.nt = (int)ceil_div(op.vocab, pl.n);
+    op.lse2 = pl.lse2;
+    op.ghat = pl.ghat;
+    op.g = static_cast<T*>(pl.g);
+    op.ldg = (int)pl.piece;
+    // f16 holds G times 2^14: the target's entry stays below its largest value
+    // and entries down to 2^-28 of the largest gradient weight stay normal numbers
+    op.gscale = format_of<T>() == 0 ? 16384.0f : 1.0f;
+    const int64_t tiles = ceil_div(a.rows, 128 * CG) * op.nt;
+    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
+    prod.v0 = (int)v0;
+    prod.width = op.vocab;
+    prod.first = v0 == 0;
+    // columns after the piece are not read: the map ends there
+    if (!mxs::gemm::make_map(&prod.g_k, pl.g, 2, prod.width, round_up(a.rows, PACK_TAIL), pl.piece, 128) ||
+        !mxs::gemm::make_map(&prod.g_m, pl.g, 2, prod.width, round_up(a.rows, PACK_TAIL), pl.piece, 64))
+        return MXS_ERR_CUDA;
+    MXS_TRY(mxs::gemm::launch(prod, a.sms / 2, a.st));
+    return MXS_OK;
+}
+
+template <typename T>
+int forward(const Call& a, const Plan& pl, float* loss, float* lse) {
+    const void* w = a.weight;
+    int64_t ldw = a.ldw;
+    if (pl.w) {
+        MXS_TRY(mxs::copy_rows(a.weight, 2 * a.ldw, pl.w, 2 * pl.ldk, a.vocab, 2 * a.d, a.sms, a.st));
+        w = pl.w, ldw = pl.ldk;
+    }
+    int rc = pack_rows<T>(a, pl, nullptr, nullptr);
+    if (rc) return rc;
+    return a.rows > 128 ? score<2, T>(a, pl, w, ldw, loss, lse) : score<1, T>(a, pl, w, ldw, loss, lse);
+}
+
+template <typename T>
+int backward(const Call& a, const Plan& pl, const float* lse, const float* grad, void* gh, int64_t ldgh, void* gw,
+             int64_t ldgw) {
+    const void* w = a.weight;
+    int64_t ldw = a.ldw;
+    if (pl.w) {
+        MXS_TRY(mxs::copy_rows(a.weight, 2 * a.ldw, pl.w, 2 * pl.ldk, a.vocab, 2 * a.d, a.sms, a.st));
+        w = pl.w, ldw = pl.ldk;
+    }
+    int rc = pack_rows<T>(a, pl, lse, grad);
+    if (rc) return rc;
+    ProductOp<T> prod{};
+    prod.format = format_of<T>();
+    prod.drop = mxs::test_drop_tile();
+    prod.status = a.status;
+    prod.head = pl.head;
+    prod.d = (int)a.d;
+    prod.n = pl.dn;
+    prod.nt = pl.dnt;
+    prod.split_width = (int)std::min(pl.piece, a.vocab);
+    prod.acc = pl.acc;
+    prod.want_h = gh != nullptr;
+    prod.want_w = gw != nullptr;
+    prod.dw = static_cast<T*>(gw);
+    prod.lddw = ldgw;
+    prod.scale = (float)(1.0 / a.temperature / (format_of<T>() == 0 ? 16384.0 : 1.0));
+    prod.vec = mxs::aligned16(gw, 2 * ldgw);
+    if (!mxs::gemm::make_map(&prod.w_n, w, 2, a.d, a.vocab, ldw, 64) ||
+        !mxs::gemm::make_map(&prod.h_n, pl.packed, 2, a.d, round_up(a.rows, PACK_TAIL), pl.ldk, 64))
+        return MXS_ERR_CUDA;
+    for (int64_t v0 = 0; v0 < a.vocab; v0 += pl.piece) {
+        rc = a.rows > 128 ? grad_piece<2, T>(a, pl, w, ldw, v0, prod) : grad_piece<1, T>(a, pl, w, ldw, v0, prod);
+        if (rc) return rc;
+    }
+    if (gh)
+        MXS_TRY(launch_dependent(grad_hidden_out_kernel<T>, (unsigned)a.rows, 256, a.st, pl.acc, pl.pos, pl.head,
+                                 (int)a.d, pl.dn, (int)std::min(pl.piece, a.vocab), a.sms / 2, prod.scale,
+                                 static_cast<T*>(gh), ldgh));
+    return MXS_OK;
 }
 
 }  // namespace
@@ -414,11 +745,14 @@ extern "C" {
 
 int mxs_ce_workspace_size(const void* d_weight, int64_t ld_weight, int64_t rows, int64_t d_model, int64_t vocab,
                           int backward, size_t* bytes) {
-    if (!bytes || rows < 0 || d_model <= 0 || vocab <= 0 || ld_weight < d_model || rows > INT32_MAX - 256 ||
-        d_model > INT32_MAX - 256 || vocab > INT32_MAX - 256)
+    if (!bytes || rows < 0 || d_model <= 0 || vocab <= 0 || ld_weight < d_model || rows > MAX_DIM ||
+        d_model > MAX_DIM || vocab > MAX_DIM)
         return MXS_ERR_INVALID;
-    (void)d_weight;
-    *bytes = make_plan(nullptr, rows, d_model, vocab, backward != 0).bytes;
+    int sms = 0;
+    uint32_t* status = nullptr;
+    const int rc = mxs::device_info(&sms, &status);
+    if (rc) return rc;
+    *bytes = make_plan(nullptr, sms, d_weight, ld_weight, rows, d_model, vocab, backward != 0).bytes;
     return MXS_OK;
 }
 
@@ -429,28 +763,13 @@ int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const void* d_we
     if (bad_shape(ld_hidden, ld_weight, dtype, rows, d_model, vocab, target_bytes, temperature)) return MXS_ERR_INVALID;
     if (rows == 0) return MXS_OK;
     if (!d_hidden || !d_weight || !d_targets) return MXS_ERR_INVALID;
-    int sms = 0;
-    uint32_t* status = nullptr;
-    int rc = mxs::device_info(&sms, &status);
+    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab, d_targets, target_bytes, temperature, 0,
+           nullptr, static_cast<cudaStream_t>(stream)};
+    const int rc = mxs::device_info(&a.sms, &a.status);
     if (rc) return rc;
-    const Plan pl = make_plan(d_workspace, rows, d_model, vocab, false);
+    const Plan pl = make_plan(d_workspace, a.sms, d_weight, ld_weight, rows, d_model, vocab, false);
     if (!mxs::workspace_ok(d_workspace, workspace_bytes, pl.bytes)) return MXS_ERR_WORKSPACE;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    Pack pk{d_hidden, ld_hidden, d_targets, target_bytes, (int)rows, (int)d_model, pl.ldk, vocab, nullptr, nullptr,
-            pl.head, pl.packed, pl.pos, pl.target, nullptr, nullptr};
-    rc = dtype == MXS_BF16 ? launch_pack<__nv_bfloat16>(pk, sms, st) : launch_pack<__half>(pk, sms, st);
-    if (rc) return rc;
-    const int tiles = (int)ceil_div(vocab, TN);
-    Score s{pl.packed, d_weight, ld_weight, (int)d_model, pl.ldk, (int)vocab, (float)(LOG2E / temperature),
-            pl.head, pl.target, pl.part, pl.ytarget, (int)rows};
-    const dim3 grid(tiles, (unsigned)ceil_div(rows, TM));
-    if (dtype == MXS_BF16)
-        score_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(s);
-    else
-        score_kernel<__half><<<grid, 256, 0, st>>>(s);
-    score_join_kernel<<<(unsigned)ceil_div(rows, 8), 256, 0, st>>>(pl.part, pl.ytarget, pl.pos, (int)rows, tiles,
-                                                                   d_loss, d_lse);
-    return cudaGetLastError() == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+    return dtype == MXS_BF16 ? forward<__nv_bfloat16>(a, pl, d_loss, d_lse) : forward<__half>(a, pl, d_loss, d_lse);
 }
 
 int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
@@ -462,61 +781,23 @@ int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const v
         (d_grad_hidden && ld_grad_hidden < d_model) || (d_grad_weight && ld_grad_weight < d_model))
         return MXS_ERR_INVALID;
     if (!d_grad_hidden && !d_grad_weight) return MXS_OK;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab, d_targets, target_bytes, temperature, 0,
+           nullptr, static_cast<cudaStream_t>(stream)};
     if (rows == 0) {  // no row: the weight's gradient is zero
-        if (d_grad_weight &&
-            cudaMemset2DAsync(d_grad_weight, 2 * ld_grad_weight, 0, 2 * d_model, vocab, st) != cudaSuccess)
-            return MXS_ERR_CUDA;
+        if (d_grad_weight)
+            MXS_TRY(cudaMemset2DAsync(d_grad_weight, 2 * ld_grad_weight, 0, 2 * d_model, vocab, a.st));
         return MXS_OK;
     }
     if (!d_hidden || !d_weight || !d_targets || !d_lse || !d_grad_loss) return MXS_ERR_INVALID;
-    int sms = 0;
-    uint32_t* status = nullptr;
-    int rc = mxs::device_info(&sms, &status);
+    const int rc = mxs::device_info(&a.sms, &a.status);
     if (rc) return rc;
-    const Plan pl = make_plan(d_workspace, rows, d_model, vocab, true);
+    const Plan pl = make_plan(d_workspace, a.sms, d_weight, ld_weight, rows, d_model, vocab, true);
     if (!mxs::workspace_ok(d_workspace, workspace_bytes, pl.bytes)) return MXS_ERR_WORKSPACE;
-    Pack pk{d_hidden, ld_hidden, d_targets, target_bytes, (int)rows, (int)d_model, pl.ldk, vocab, d_lse, d_grad_loss,
-            pl.head, pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat};
-    rc = dtype == MXS_BF16 ? launch_pack<__nv_bfloat16>(pk, sms, st) : launch_pack<__half>(pk, sms, st);
-    if (rc) return rc;
-    // f16 holds G times 2^14: the target's entry stays below its largest value
-    // and probabilities down to 2^-28 stay normal numbers
-    const float gscale = dtype == MXS_F16 ? 16384.0f : 1.0f;
-    Grad g{};
-    g.h = pl.packed, g.w = d_weight, g.ldw = ld_weight, g.d = (int)d_model, g.ldk = pl.ldk, g.vocab = (int)vocab;
-    g.ldg = pl.ldg, g.c = (float)(LOG2E / temperature), g.inv_t = (float)(1.0 / temperature), g.head = pl.head;
-    g.target = pl.target, g.lse2 = pl.lse2, g.ghat = pl.ghat, g.g = pl.g, g.acc = pl.acc;
-    g.dw = d_grad_weight, g.lddw = ld_grad_weight, g.gscale = gscale, g.inv_gscale = 1.0f / gscale;
-    for (int64_t v0 = 0; v0 < vocab; v0 += pl.ldg) {
-        g.v0 = (int)v0;
-        g.width = (int)std::min<int64_t>(pl.ldg, vocab - v0);
-        g.first = v0 == 0;
-        const unsigned gm = (unsigned)ceil_div(rows, TM), gv = (unsigned)ceil_div(g.width, TN),
-                       gd = (unsigned)ceil_div(d_model, TN);
-        const bool bf = dtype == MXS_BF16;
-        auto go = [&](auto kb, auto kh, dim3 grid) {
-            if (bf)
-                kb<<<grid, 256, 0, st>>>(g);
-            else
-                kh<<<grid, 256, 0, st>>>(g);
-        };
-        go(grad_logits_kernel<__nv_bfloat16>, grad_logits_kernel<__half>, dim3(gv, gm));
-        if (d_grad_hidden) go(grad_hidden_kernel<__nv_bfloat16>, grad_hidden_kernel<__half>, dim3(gd, gm));
-        if (d_grad_weight) go(grad_weight_kernel<__nv_bfloat16>, grad_weight_kernel<__half>, dim3(gd, gv));
-    }
-    if (d_grad_hidden) {
-        const float sc = g.inv_t * g.inv_gscale;
-        if (dtype == MXS_BF16)
-            grad_hidden_out_kernel<<<(unsigned)rows, 256, 0, st>>>(pl.acc, pl.pos, pl.head, (int)d_model, sc,
-                                                                   static_cast<__nv_bfloat16*>(d_grad_hidden),
-                                                                   ld_grad_hidden);
-        else
-            grad_hidden_out_kernel<<<(unsigned)rows, 256, 0, st>>>(pl.acc, pl.pos, pl.head, (int)d_model, sc,
-                                                                   static_cast<__half*>(d_grad_hidden),
-                                                                   ld_grad_hidden);
-    }
-    return cudaGetLastError() == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+    return dtype == MXS_BF16
+               ? backward<__nv_bfloat16>(a, pl, d_lse, d_grad_loss, d_grad_hidden, ld_grad_hidden, d_grad_weight,
+                                         ld_grad_weight)
+               : backward<__half>(a, pl, d_lse, d_grad_loss, d_grad_hidden, ld_grad_hidden, d_grad_weight,
+                                  ld_grad_weight);
 }
 
 }  // extern "C"

@@ -1,0 +1,423 @@
+// The tensor-core frame of the output-head operators: a persistent,
+// warp-specialised sm_100a kernel body that an Op fills in.
+//
+//   warp 0      loads operand tiles (TMA, 128-byte swizzle) into a ring of stages
+//   warp 1      issues tcgen05.mma (one thread), accumulators in TMEM
+//   warps 2..9  read accumulators back (tcgen05.ld) and do the Op's epilogue
+//
+// A tile is 128 rows per CTA by up to 256 columns. With CG = 2 a pair of CTAs
+// works on one 256-row tile: each loads its 128 rows of A and half of B's
+// columns, the even CTA issues the pair's MMAs, and every operand byte crosses
+// L2 -> shared memory once for 256 x 256 outputs (64 bytes per clock and SM at
+// full MMA rate, against 96 for a single CTA's 128 x 256, which L2 does not
+// deliver). TMEM's 512 columns hold two accumulators, so the epilogue of one
+// tile runs under the products of the next.
+//
+// Operands are held with 128 bytes of the contiguous direction per row, either
+// along K ("K-major": 64 16-bit or 128 8-bit values of K in a row) or along the
+// tile's own direction ("MN-major": 64 values of M or N in a row, one row per k),
+// so all three products of a loss and its gradients read the same row-major
+// matrices without a transposed copy.
+//
+// Every wait is bounded (about 1 s, as in the streaming kernel); a wait that
+// gives up marks the CTA dead, its roles stop, copies and MMAs in flight are
+// waited for (bounded again), TMEM is freed, and the device's status word gets
+// FLAG_TIMEOUT. No TMA multicast anywhere.
+#pragma once
+#include <atomic>
+
+#include <cuda.h>
+
+#include "mxs_common.cuh"
+
+namespace mxs {
+namespace gemm {
+
+constexpr int THREADS = 320;
+constexpr int EPI_WARPS = 8;
+constexpr int A_BYTES = 128 * 128;
+constexpr int ROW = 128;  // bytes of a stage row (one swizzle row)
+
+template <int CG>
+struct Geo {
+    static constexpr int B_BYTES = 256 / CG * ROW;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 196608 / STAGE;  // 192 KB: 4 or 6
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 1024;
+};
+
+struct Tile {
+    int m0, n0;   // first row and column of the pair's (or CTA's) tile, in the Op's own terms
+    int k0, kn;   // first k block and number of blocks
+    int n;        // columns of the MMA
+    int kind;     // Op's own
+};
+
+struct Ring {
+    uint64_t full[6], empty[6], tfull[2], tempty[2], drain;
+    uint32_t tmem;
+    int dead;
+};
+
+// --- PTX ---------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 2-D tile load; `bar` is a shared::cluster address (with CG = 2, the even CTA's barrier).
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
+    if (CG == 2)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+    else
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+    if (CG == 2) {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base));
+    } else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(base));
+    }
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Arrives on `bar` (of both CTAs of the pair) when every MMA issued so far has finished.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    if (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                     : "memory");
+}
+
+template <int CG, bool F8>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    const uint32_t p = add;
+    if (F8) {
+        if (CG == 2)
+            asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                         " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+                         "r"(idesc), "r"(p) : "memory");
+        else
+            asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                         " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+                         "r"(idesc), "r"(p) : "memory");
+    } else {
+        if (CG == 2)
+            asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                         " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+                         "r"(idesc), "r"(p) : "memory");
+        else
+            asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                         " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+                         "r"(idesc), "r"(p) : "memory");
+    }
+}
+
+// 32 accumulator columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        " tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle: start address, leading and
+// stride byte offsets (all in 16-byte units), descriptor version 1.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+
+// Instruction descriptor: fp32 accumulators, operand formats, majors, shape.
+// Formats: kind::f16 0 = f16, 1 = bf16; kind::f8f6f4 0 = e4m3.
+__device__ __forceinline__ uint32_t instr_desc(int format, bool a_mn, bool b_mn, int m, int n) {
+    return 1u << 4 | (uint32_t)format << 7 | (uint32_t)format << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 |
+           (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+// --- waits -------------------------------------------------------------------
+
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+// False (and the CTA is dead) when the limit ran out or another role gave up.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ring* ring) {
+    if (try_wait_cluster(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!try_wait_cluster(bar, parity)) {
+        if (*(volatile int*)&ring->dead) return false;
+        if (globaltimer_ns() - t0 > 1000000000ull) {
+            *(volatile int*)&ring->dead = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// What an Op needs to know of where it runs.
+struct Ctx {
+    int units, unit;   // CTAs or pairs in the grid, and this one
+    uint32_t rank;     // CTA's place in its pair
+    int kept;          // Op's row count, read on the device
+};
+
+// The kernel body. Op (a __grid_constant__ parameter) has
+//   CG, F8, PROMOTE        compile-time: CTAs per tile, 8-bit operands, join accumulators per k block
+//   format                 operand format of the instruction descriptor
+//   drop                   test hook: CTA 0's producer stops before this block (-1: off)
+//   status                 the device's status word
+//   prefetch()             tensor-map prefetch
+//   kept()                 the row count
+//   tile(i, ctx, tile)     i-th tile of this unit, false when there is none
+//   a_mn(t), b_mn(t)       operand majors of a tile
+//   bytes(t)               bytes this CTA loads per block
+//   load(t, kb, sa, sb, bar, ctx)
+//   zero(t, row, half, ctx)                                    the epilogue of a tile without blocks
+//   epilogue(t, tmem, row, half, ctx)                          !PROMOTE
+//   Acc, begin(...), join(...), finish(...)                    PROMOTE
+template <typename Op>
+__device__ __forceinline__ void run(const Op& op) {
+    constexpr int CG = Op::CG;
+    using G = Geo<CG>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    Ring* ring = reinterpret_cast<Ring*>(base + (size_t)G::STAGES * G::STAGE);
+    const uint32_t stages = smem_u32(base);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Ctx ctx;
+    ctx.rank = CG == 2 ? cluster_rank() : 0;
+    ctx.units = gridDim.x / CG;
+    ctx.unit = blockIdx.x / CG;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G::STAGES; ++i) {
+            mbar_init(&ring->full[i], 1);
+            mbar_init(&ring->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ring->tfull[i], 1);
+            mbar_init(&ring->tempty[i], EPI_WARPS * CG);
+        }
+        mbar_init(&ring->drain, 1);
+        ring->dead = 0;
+        fence_mbar_init();
+        op.prefetch();
+    }
+    if (warp == 1) tmem_alloc<CG>(&ring->tmem);
+    fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync();
+    fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)&ring->tmem;
+    grid_wait();
+    grid_launch_dependents();
+    ctx.kept = op.kept();
+
+    Tile t;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            int64_t issued = 0;
+            bool ok = true;
+            for (int i = 0; ok && op.tile(i, ctx, t); ++i)
+                for (int kb = 0; kb < t.kn; ++kb) {
+                    if (!wait(&ring->empty[s], ph ^ 1, ring)) { ok = false; break; }
+                    if (op.drop >= 0 && blockIdx.x == 0 && issued >= op.drop) { ok = false; break; }
+                    uint32_t bar = smem_u32(&ring->full[s]);
+                    if (ctx.rank == 0) mbar_arrive_expect_tx(&ring->full[s], CG * op.bytes(t));
+                    if (CG == 2) bar = map_to_rank(bar, 0);
+                    const uint32_t sa = stages + s * G::STAGE;
+                    op.load(t, t.k0 + kb, sa, sa + A_BYTES, bar, ctx);
+                    ++issued;
+                    if (++s == G::STAGES) s = 0, ph ^= 1;
+                }
+            // gave up: the copies still in flight (at most one per stage) land before the CTA ends
+            if (!ok && ctx.rank == 0) {
+                const int64_t n = issued < G::STAGES ? issued : (int64_t)G::STAGES;
+                for (int64_t j = issued - n; j < issued; ++j)
+                    mbar_wait_bounded(&ring->full[j % G::STAGES], (uint32_t)(j / G::STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && ctx.rank == 0) {
+            uint32_t s = 0, ph = 0, buf = 0, tph = 0;
+            bool ok = true;
+            for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
+                const bool amn = op.a_mn(t), bmn = op.b_mn(t);
+                const uint32_t idesc = instr_desc(op.format, amn, bmn, 128 * CG, t.n);
+                // K-major: 8-row groups 1024 bytes apart, a step of K is 32 bytes of the row.
+                // MN-major: 64-wide slabs of 64 k rows (8192 bytes), 8-k groups 1024 bytes
+                // apart, a step of 16 k rows is 2048 bytes.
+                const uint64_t step_a = (amn ? 2048 : 32) >> 4, step_b = (bmn ? 2048 : 32) >> 4;
+                for (int kb = 0; kb < t.kn; ++kb) {
+                    if (Op::PROMOTE || kb == 0) {
+                        if (!wait(&ring->tempty[buf], tph ^ 1, ring)) { ok = false; break; }
+                        fence_after();
+                    }
+                    if (!wait(&ring->full[s], ph, ring)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t sa = stages + s * G::STAGE;
+                    uint64_t da = smem_desc(sa, amn ? 8192 : 16, 1024);
+                    uint64_t db = smem_desc(sa + A_BYTES, bmn ? 8192 : 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        mma<CG, Op::F8>(tmem + buf * 256, da, db, idesc, k > 0 || (!Op::PROMOTE && kb > 0));
+                        da += step_a;
+                        db += step_b;
+                    }
+                    commit<CG>(&ring->empty[s]);
+                    if (++s == G::STAGES) s = 0, ph ^= 1;
+                    if (Op::PROMOTE || kb == t.kn - 1) {
+                        commit<CG>(&ring->tfull[buf]);
+                        if (++buf == 2) buf = 0, tph ^= 1;
+                    }
+                }
+            }
+            if (!ok) {  // MMAs in flight finish before TMEM is freed
+                commit<CG>(&ring->drain);
+                mbar_wait_bounded(&ring->drain, 0);
+            }
+        }
+    } else {
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        const int row = (int)ctx.rank * 128 + quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t te0 = CG == 2 ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
+        uint32_t buf = 0, tph = 0;
+        bool ok = true;
+        for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
+            if (t.kn == 0) {  // an empty sum: no product, no accumulator
+                op.zero(t, row, half, ctx);
+                continue;
+            }
+            if constexpr (Op::PROMOTE) {
+                typename Op::Acc acc;
+                op.begin(acc, t, row, half, ctx);
+                for (int kb = 0; kb < t.kn; ++kb) {
+                    op.prepare(acc, t, t.k0 + kb, row, half, ctx);
+                    ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
+                    if (!ok) break;
+                    fence_after();
+                    op.join(acc, t, tmem + buf * 256 + lanes, row, half, ctx);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_remote(te0 + buf * 8);
+                    if (++buf == 2) buf = 0, tph ^= 1;
+                }
+                if (ok) op.finish(acc, t, row, half, ctx);
+            } else {
+                ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
+                if (!ok) break;
+                fence_after();
+                op.epilogue(t, tmem + buf * 256 + lanes, row, half, ctx);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_remote(te0 + buf * 8);
+                if (++buf == 2) buf = 0, tph ^= 1;
+            }
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync();
+    fence_after();
+    if (warp == 1) tmem_free<CG>(tmem);
+    if (threadIdx.x == 0 && ring->dead) atomicOr(op.status, FLAG_TIMEOUT);
+}
+
+// --- host --------------------------------------------------------------------
+
+// A row-major [rows][cols] matrix of 1- or 2-byte elements, read in boxes of
+// 128 bytes by box_rows rows, 128-byte swizzle; what lies outside reads zero.
+// False when the encoder is missing or refuses.
+bool make_map(CUtensorMap* map, const void* base, int elem_bytes, int64_t cols, int64_t rows, int64_t ld, int box_rows);
+
+template <typename Op>
+__global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Op op) {
+    run(op);
+}
+
+// Launches the Op on units * CG CTAs, allowed to start while the kernel before it
+// on the stream drains (it waits on the device).
+template <typename Op>
+cudaError_t launch(const Op& op, int units, cudaStream_t st) {
+    constexpr int CG = Op::CG;
+    static std::atomic<uint64_t> configured{0};  // a bit for each device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (!(configured.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<CG>::SMEM);
+        if (e != cudaSuccess) return e;
+        configured.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(units * CG);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Geo<CG>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CG;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel<Op>, op);
+}
+
+}  // namespace gemm
+}  // namespace mxs

@@ -48,4 +48,15 @@ inline bool workspace_ok(const void* ws, size_t bytes, size_t need) {
     return need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 256 == 0 && bytes >= need);
 }
 
+// Rows of `row_bytes` bytes into aligned rows of ld_to bytes, a warp each.
+__global__ void copy_rows_kernel(const uint8_t* from, int64_t ld_from, uint8_t* to, int64_t ld_to, int64_t rows,
+                                 int64_t row_bytes);
+cudaError_t copy_rows(const void* from, int64_t ld_from, void* to, int64_t ld_to, int64_t rows, int64_t row_bytes,
+                      int sms, cudaStream_t st);
+
+// Tile width for `n` columns: the multiple of `step` in [lo, 256] whose
+// rounds of tiles over the units cost least, a round costing its width and a
+// fixed part (filling and draining a tile's pipeline, worth about 16 columns).
+int tile_width(int64_t m_tiles, int64_t n, int units, int lo, int step);
+
 }  // namespace mxs

@@ -12,6 +12,7 @@ cudaError_t sample_kernel_launch(const Params& p, int grid, bool tma, cudaStream
 int workspace_zero_prefix(size_t* bytes);  // mxs_api.cu
 // SM count and status word of the current device (MXS_OK, or the error current_device gives); mxs_api.cu
 int device_info(int* sms, uint32_t** status);
+int64_t test_drop_tile();  // mxs_set_test_hooks' drop_tile; mxs_api.cu
 
 // The row lists a vocab-sharded shard step leaves in the library workspace
 // (two-kernel path only): every logit of a chunk's later tiles above a
