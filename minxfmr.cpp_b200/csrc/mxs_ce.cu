@@ -188,6 +188,7 @@ template <int CG_>
 struct LogitTiles {
     static constexpr int CG = CG_;
     static constexpr bool F8 = false, PROMOTE = false;
+    __device__ int group() const { return INT32_MAX; }
     CUtensorMap mh, mw;
     int format;
     int64_t drop;
@@ -224,20 +225,48 @@ struct LogitTiles {
 // Each thread holds half a tile's columns of one row: the largest y of the others
 // and sum 2^(y - largest). The exponentials run at 16 a clock and SM: 2048 clocks
 // for 128 x 256, under the 512 clocks of each 64 of d_model that the products take.
+// The MMA's own fp32 sum rounds towards zero at every 16 products, which at
+// d_model 3584 leaves 2e-6 of the logits' size; joining the accumulator in
+// registers (round to nearest) every 1024 products keeps it below 1e-6 and costs
+// one more read of the accumulator for each.
 template <int CG_>
 struct ScoreOp : LogitTiles<CG_> {
+    static constexpr bool PROMOTE = true;
+    __device__ int group() const { return 16; }
+    struct Acc {
+        float v[4][32];
+    };
     float2* part;    // [tile * 2 + half][rows]
     float* ytarget;  // [rows]
 
-    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
+    __device__ void begin(Acc& a, const Tile&, int, int, const Ctx&) const {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) a.v[i / 32][i % 32] = 0.0f;
+    }
+    __device__ void prepare(Acc&, const Tile&, int, int, int, const Ctx&) const {}
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
+        if (((t.m0 + row) & ~31) >= x.kept) return;  // no row of this warp
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = half * 32 + i * 64;
+            if (c0 >= t.n) break;
+            float v[32];
+            mxs::gemm::tmem_ld32(tmem + c0, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a.v[i][j] += v[j];
+        }
+    }
+    __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx& x) const {
         const int r = t.m0 + row;
-        if ((r & ~31) >= x.kept) return;  // no row of this warp
+        if ((r & ~31) >= x.kept) return;
         const int hit = r < x.kept ? this->target[r] - t.n0 : -1;  // the target's column of this tile
         const int cols = min(t.n, this->vocab - t.n0);
         float m = -INFINITY, s = 0.0f;
-        for (int c0 = half * 32; c0 < t.n; c0 += 64) {
-            float v[32];
-            mxs::gemm::tmem_ld32(tmem + c0, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = half * 32 + i * 64;
+            if (c0 >= t.n) break;
+            float(&v)[32] = a.v[i];
             if (hit >= c0 && hit < c0 + 32) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
@@ -304,33 +333,6 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, con
     }
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half*) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// 32 values to `out`, as 16-byte stores where `vec` says that they are aligned.
-template <typename T>
-__device__ __forceinline__ void store32(T* out, const float (&v)[32], int n, bool vec) {
-    if (vec && n >= 32) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-            T* tag = nullptr;
-            *reinterpret_cast<uint4*>(out + j) =
-                make_uint4(pack2(v[j], v[j + 1], tag), pack2(v[j + 2], v[j + 3], tag), pack2(v[j + 4], v[j + 5], tag),
-                           pack2(v[j + 6], v[j + 7], tag));
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < n) out[j] = mxs::from_f32<T>(v[j]);
-    }
-}
-
 // The logits of a piece again, left as G = ghat (softmax - hot) in the operands'
 // type (rounded once; the products that read it accumulate in fp32). Rows after
 // the last kept one and columns after the piece read zero.
@@ -367,7 +369,7 @@ struct GradLogitsOp : LogitTiles<CG_> {
                 for (int j = 0; j < 32; ++j)
                     if (c0 + j >= cols) v[j] = 0.0f;
             }
-            store32(out + c0, v, ldg - t.n0 - c0, true);
+            mxs::store32(out + c0, v, ldg - t.n0 - c0, true);
         }
     }
 };
@@ -380,6 +382,7 @@ template <typename T>
 struct ProductOp {
     static constexpr int CG = 2;
     static constexpr bool F8 = false, PROMOTE = false;
+    __device__ int group() const { return INT32_MAX; }
     CUtensorMap g_k, g_m, w_n, h_n;
     int format;
     int64_t drop;
@@ -475,7 +478,7 @@ struct ProductOp {
             mxs::gemm::tmem_ld32(tmem + c0, v);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= s;
-            if (m < width) store32(out + c0, v, d - t.n0 - c0, vec);
+            if (m < width) mxs::store32(out + c0, v, d - t.n0 - c0, vec);
         }
     }
     __device__ void zero(const Tile& t, int row, int half, const Ctx&) const {

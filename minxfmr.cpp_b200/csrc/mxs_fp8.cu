@@ -6,6 +6,7 @@
 
 #include <cuda_fp8.h>
 
+#include "mxs_gemm.cuh"
 #include "mxs_head.cuh"
 #include "mxs_launch.h"
 
@@ -14,6 +15,8 @@ namespace {
 using mxs::Carve;
 using mxs::ceil_div;
 using mxs::round_up;
+using mxs::gemm::Ctx;
+using mxs::gemm::Tile;
 using mxs::to_f32;
 
 constexpr int BLK = 128;
@@ -22,104 +25,314 @@ constexpr float FP8_MAX = 448.0f;
 __device__ __forceinline__ float block_scale(float top) {
     return top > 0.0f ? fmaxf(top / FP8_MAX, 1.17549435e-38f) : 1.0f;
 }
-__device__ __forceinline__ uint8_t to_fp8(float x) {
-    return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+
+// Eight values of a row, as 16-byte loads where they are aligned and whole.
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], const __nv_bfloat16*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
 }
-__device__ __forceinline__ float from_fp8(uint8_t x) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3)));
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], const __half*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* x, int n, bool vec, float (&v)[8]) {
+    if (vec && n >= 8) {
+        unpack(*reinterpret_cast<const uint4*>(x), v, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(x[i]) : 0.0f;
+    }
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* x, int n, bool vec, float (&v)[8]) {
+    if (vec && n >= 8) {
+        const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? x[i] : 0.0f;
+    }
 }
 
-// One CTA of 256 threads per block: its largest finite magnitude, then its values.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols,
-                                                       int block_rows, uint8_t* q, int64_t ldq, float* scale) {
-    __shared__ float s_max[8];
-    const int64_t c0 = (int64_t)blockIdx.x * BLK, r0 = (int64_t)blockIdx.y * block_rows;
-    const int64_t nr = min((int64_t)block_rows, rows - r0), nc = min((int64_t)BLK, cols - c0);
-    float top = 0.0f;
-    for (int i = threadIdx.x; i < block_rows * BLK; i += 256) {
-        const int r = i / BLK, c = i % BLK;
-        if (r < nr && c < nc) {
-            const float v = fabsf(to_f32(x[(r0 + r) * ldx + c0 + c]));
-            if (v <= FLT_MAX) top = fmaxf(top, v);
+// The largest magnitude: NaN does not count; `all` keeps infinities in.
+__device__ __forceinline__ float top8(const float (&v)[8], bool all) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(v[i]);
+        if (all || a <= FLT_MAX) m = fmaxf(m, a);
+    }
+    return m;
+}
+
+// x / s rounded to nearest, from r = 1 / s rounded to nearest: Markstein's
+// theorem (IBM J. Res. Dev. 34, 1990) makes q + r (x - q s) the correctly rounded
+// quotient for q = x r, as long as the remainder is exact. It is for s >= 2^-90
+// and quotients of at least 2^-11; smaller ones round to zero in 8 bits either
+// way. Smaller scales (`slow`) divide.
+__device__ __forceinline__ float quotient(float x, float s, float r, bool slow) {
+    if (slow) return x / s;
+    const float q = x * r;
+    return fmaf(fmaf(-q, s, x), r, q);
+}
+__device__ __forceinline__ uint32_t quad(const float* y) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+__device__ __forceinline__ void store8(uint8_t* q, int n, bool vec, const float (&v)[8], float s, float r, bool slow) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = quotient(v[i], s, r, slow);
+    const uint2 w = make_uint2(quad(y), quad(y + 4));
+    if (vec && n >= 8) {
+        *reinterpret_cast<uint2*>(q) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) q[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    }
+}
+
+// Bound by memory: each value is read once and kept in registers between its
+// block's maximum and its rounding. ROWS_OF = 1: sixteen lanes hold a block of
+// 128, a warp two neighbouring ones, twice. ROWS_OF = 128: a CTA of 256 threads
+// holds a block, sixteen lanes a row, eight rows each.
+template <typename T, int ROWS_OF>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols, uint8_t* q,
+                                                       int64_t ldq, float* scale, bool vec_in, bool vec_out) {
+    constexpr int HELD = ROWS_OF == 1 ? 2 : 8;
+    const int tid = threadIdx.x, lane = tid & 31, sub = tid & 15;
+    const int64_t bc = ceil_div(cols, BLK);
+    int64_t row[HELD], col[HELD];
+    if (ROWS_OF == 1) {
+        const int64_t per_row = ceil_div(bc, 4);
+        const int64_t task = (int64_t)blockIdx.x * 8 + (tid >> 5);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            row[i] = task / per_row;
+            col[i] = (task % per_row) * (4 * BLK) + i * (2 * BLK) + lane * 8;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            row[i] = (int64_t)(blockIdx.x / bc) * BLK + i * 16 + (tid >> 4);
+            col[i] = (int64_t)(blockIdx.x % bc) * BLK + sub * 8;
         }
     }
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_max[w]);
-    const float s = block_scale(top);
-    if (threadIdx.x == 0) scale[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
-    for (int i = threadIdx.x; i < block_rows * BLK; i += 256) {
-        const int r = i / BLK, c = i % BLK;
-        if (r < nr && c < nc) q[(r0 + r) * ldq + c0 + c] = to_fp8(to_f32(x[(r0 + r) * ldx + c0 + c]) / s);
+    float v[HELD][8];
+    int n[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        n[i] = row[i] < rows ? (int)min((int64_t)8, cols - col[i]) : 0;  // may be negative: nothing
+        load8(x + (n[i] > 0 ? row[i] * ldx + col[i] : 0), n[i], vec_in, v[i]);
+    }
+    __shared__ float s_top[8];
+    float s[HELD];
+    for (int pass = 0; pass < 2; ++pass) {  // the second pass leaves infinities out, where there are any
+        float top = 0.0f;
+        bool inf = false;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const float mine = top8(v[i], pass == 0);
+            top = ROWS_OF == 1 ? mine : fmaxf(top, mine);
+            if (ROWS_OF == 1 || i == HELD - 1) {
+#pragma unroll
+                for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (ROWS_OF != 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    if (lane == 0) s_top[tid >> 5] = top;
+                    __syncthreads();
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+                    __syncthreads();
+                }
+                inf |= top > FLT_MAX;
+                s[i] = top;
+            }
+        }
+        // ROWS_OF 1: any block of the warp; 128: the same for the whole CTA
+        if (!__any_sync(0xffffffffu, inf)) break;
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const float sc = block_scale(s[ROWS_OF == 1 ? i : HELD - 1]);
+        const float r = 1.0f / sc;
+        // 2^-90; an infinity would spoil its own remainder
+        const bool slow = sc < 8.0779357e-28f || top8(v[i], true) > FLT_MAX;
+        if (n[i] > 0) {
+            store8(q + row[i] * ldq + col[i], n[i], vec_out, v[i], sc, r, slow);
+            if (ROWS_OF == 1 && sub == 0) scale[row[i] * bc + col[i] / BLK] = sc;
+        }
+        if (ROWS_OF != 1 && i == 0 && tid == 0) scale[blockIdx.x] = sc;
     }
 }
 
-struct Mat {
-    const uint8_t *a, *b;
-    int64_t lda, ldb;
+template <typename T>
+cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int br, void* q, int64_t ldq,
+                            float* scale, cudaStream_t st) {
+    const int64_t bc = ceil_div(cols, BLK);
+    const bool vin = mxs::aligned16(x, ldx * (int64_t)sizeof(T));
+    const bool vout = reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+    const T* xt = static_cast<const T*>(x);
+    uint8_t* qt = static_cast<uint8_t*>(q);
+    // runs of rows whose CTAs a grid can count
+    const int64_t per = br == 1 ? ceil_div(bc, 4) : bc;      // tasks in a row of blocks
+    const int64_t most = std::max<int64_t>(1, ((int64_t)INT32_MAX - 8) / per) * br;
+    for (int64_t r = 0; r < rows; r += most) {
+        const int64_t n = std::min(most, rows - r);
+        float* sc = scale + r / br * bc;
+        if (br == 1)
+            quantize_kernel<T, 1><<<(unsigned)ceil_div(n * per, 8), 256, 0, st>>>(xt + r * ldx, ldx, n, cols,
+                                                                                 qt + r * ldq, ldq, sc, vin, vout);
+        else
+            quantize_kernel<T, 128><<<(unsigned)(ceil_div(n, BLK) * per), 256, 0, st>>>(
+                xt + r * ldx, ldx, n, cols, qt + r * ldq, ldq, sc, vin, vout);
+    }
+    return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// The product. A stage of the ring is one block of 128 of K (128 bytes of a
+// row), so the accumulator of one block is one group: it is read back, scaled
+// by a_scale * b_scale and added in registers while the MMAs of the next block
+// fill the other accumulator (512 clocks of MMA for a 128 x 256 block, against
+// 256 of accumulator reads and 256 of FMA a scheduler).
+// ---------------------------------------------------------------------------
+
+template <int CG_, typename O>
+struct MatmulOp {
+    static constexpr int CG = CG_;
+    static constexpr bool F8 = true, PROMOTE = true;
+    __device__ int group() const { return 1; }
+    struct Acc {
+        float v[4][32];
+        float row_next, next[4], now[4];  // scales of the next block and of this one
+    };
+    CUtensorMap ma, mb;
+    int format;
+    int64_t drop;
+    uint32_t* status;
     const float *sa, *sb;
-    int rows, n, k, kb;
-    void* out;
+    int rows, cols, kb, mt, nt, n, a_rows;
+    O* out;
     int64_t ldo;
+    bool vec;
+
+    __device__ void prefetch() const {
+        mxs::gemm::prefetch_map(&ma);
+        mxs::gemm::prefetch_map(&mb);
+    }
+    __device__ int kept() const { return rows; }
+    __device__ bool tile(int i, const Ctx& x, Tile& t) const {
+        const int64_t idx = x.unit + (int64_t)i * x.units;
+        if (idx >= (int64_t)mt * nt) return false;
+        const int m = (int)(idx % mt), v = (int)(idx / mt);
+        t = Tile{m * 128 * CG, v * n, 0, kb, n, v};
+        return true;
+    }
+    __device__ bool a_mn(const Tile&) const { return false; }
+    __device__ bool b_mn(const Tile&) const { return false; }
+    __device__ uint32_t bytes(const Tile&) const { return (uint32_t)(a_rows + n / CG) * 128; }
+    __device__ void load(const Tile& t, int k, uint32_t s_a, uint32_t s_b, uint32_t bar, const Ctx& x) const {
+        mxs::gemm::tma_load<CG>(s_a, &ma, k * BLK, t.m0 + (int)x.rank * 128, bar);
+        mxs::gemm::tma_load<CG>(s_b, &mb, k * BLK, t.n0 + (int)x.rank * (n / CG), bar);
+    }
+    __device__ void zero(const Tile&, int, int, const Ctx&) const {}
+    __device__ void fetch(Acc& a, const Tile& t, int k, int row, int half) const {
+        const float s = sa[(int64_t)min(rows - 1, t.m0 + row) * kb + k];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = min(cols - 1, t.n0 + half * 32 + i * 64);  // 32 columns lie in one block of 128
+            a.next[i] = sb[(int64_t)(c0 / BLK) * kb + k];
+        }
+        a.row_next = s;
+    }
+    __device__ void begin(Acc& a, const Tile& t, int row, int half, const Ctx&) const {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) a.v[i / 32][i % 32] = 0.0f;
+        fetch(a, t, 0, row, half);
+    }
+    __device__ void prepare(Acc& a, const Tile& t, int k, int row, int half, const Ctx&) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a.now[i] = a.row_next * a.next[i];
+        if (k + 1 < kb) fetch(a, t, k + 1, row, half);
+    }
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx&) const {
+        if (((t.m0 + row) & ~31) >= rows) return;  // no row of this warp
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = half * 32 + i * 64;
+            if (c0 >= t.n) break;
+            float v[32];
+            mxs::gemm::tmem_ld32(tmem + c0, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(v[j], a.now[i], a.v[i][j]);
+        }
+    }
+    __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx&) const {
+        const int r = t.m0 + row;
+        if (r >= rows) return;
+        O* o = out + (int64_t)r * ldo + t.n0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = half * 32 + i * 64;
+            if (c0 >= t.n) break;
+            mxs::store32(o + c0, a.v[i], cols - t.n0 - c0, vec);
+        }
+    }
 };
 
-constexpr int TM = 64, TN = 64, TK = 16;
-
-template <typename O>
-__global__ void __launch_bounds__(256) matmul_kernel(const Mat p) {
-    __shared__ float sa[TK][TM + 4], sb[TK][TN + 4];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN;
-    float acc[4][4] = {};
-    for (int kb = 0; kb < p.kb; ++kb) {
-        float blk[4][4] = {};
-        for (int k0 = kb * BLK; k0 < min(p.k, (kb + 1) * BLK); k0 += TK) {
-            __syncthreads();
-            for (int i = tid; i < TM * TK; i += 256) {
-                const int k = i % TK, m = i / TK;
-                const bool in = k0 + k < p.k;
-                sa[k][m] = in && m0 + m < p.rows ? from_fp8(p.a[(int64_t)(m0 + m) * p.lda + k0 + k]) : 0.0f;
-                sb[k][m] = in && n0 + m < p.n ? from_fp8(p.b[(int64_t)(n0 + m) * p.ldb + k0 + k]) : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < TK; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) blk[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], blk[i][j]);
-        }
-        const float s1 = p.sb[(int64_t)(n0 / BLK) * p.kb + kb];
-        for (int i = 0; i < 4; ++i) {
-            const int r = min(p.rows - 1, m0 + ty * 4 + i);
-            const float s = p.sa[(int64_t)r * p.kb + kb] * s1;
-            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(blk[i][j], s, acc[i][j]);
-        }
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (r < p.rows && n < p.n) static_cast<O*>(p.out)[(int64_t)r * p.ldo + n] = mxs::from_f32<O>(acc[i][j]);
-        }
-}
-
-template <typename T>
-void launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int br, void* q, int64_t ldq, float* scale,
-                     cudaStream_t st) {
-    const int64_t gy = ceil_div(rows, br);
-    // grid rows are limited to 65535: take the rows in runs of whole blocks
-    for (int64_t y = 0; y < gy; y += 65535) {
-        const int64_t r = y * br;
-        quantize_kernel<T><<<dim3((unsigned)ceil_div(cols, BLK), (unsigned)std::min<int64_t>(65535, gy - y)), 256, 0,
-                             st>>>(static_cast<const T*>(x) + r * ldx, ldx, rows - r, cols, br,
-                                   static_cast<uint8_t*>(q) + r * ldq, ldq, scale + y * ceil_div(cols, BLK));
-    }
+template <int CG, typename O>
+int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
+                  int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
+    MatmulOp<CG, O> op{};
+    op.format = 0;
+    op.drop = mxs::test_drop_tile();
+    op.status = status;
+    op.sa = sa, op.sb = sb;
+    op.rows = (int)rows, op.cols = (int)n, op.kb = (int)ceil_div(k, BLK);
+    op.mt = (int)ceil_div(rows, 128 * CG);
+    op.n = mxs::tile_width(op.mt, n, sms / CG, 64, 32);
+    op.nt = (int)ceil_div(n, op.n);
+    op.a_rows = CG == 1 ? (int)round_up(rows, 8) : 128;
+    op.out = static_cast<O*>(out);
+    op.ldo = ldo;
+    op.vec = mxs::aligned16(out, ldo * (int64_t)sizeof(O));
+    if (!mxs::gemm::make_map(&op.ma, a, 1, k, rows, lda, op.a_rows) ||
+        !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, op.n / CG))
+        return MXS_ERR_CUDA;
+    const int64_t tiles = (int64_t)op.mt * op.nt;
+    return mxs::gemm::launch(op, (int)std::min<int64_t>(sms / CG, tiles), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
 }
 
 bool bad_type(int t) { return t != MXS_BF16 && t != MXS_F16 && t != MXS_F32; }
-constexpr int64_t LIMIT = INT32_MAX - 256;
+constexpr int64_t LIMIT = INT32_MAX - 1024;
+
+// Aligned copies of the operands that need one.
+struct Copies {
+    void *a, *b;
+    size_t bytes;
+};
+Copies copies(void* ws, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t n, int64_t k) {
+    Carve c(ws);
+    const int64_t ldk = round_up(k, 16);
+    Copies r{};
+    if (!mxs::aligned16(a, lda)) r.a = c.take<uint8_t>((size_t)rows * ldk);
+    if (!mxs::aligned16(b, ldb)) r.b = c.take<uint8_t>((size_t)n * ldk);
+    r.bytes = c.used;
+    return r;
+}
 
 // Workspace of mxs_sample_from_hidden_fp8.
 struct SamplePlan {
@@ -168,22 +381,18 @@ int mxs_quantize_fp8(const void* d_x, int64_t ld_x, int dtype, int64_t rows, int
     int rc = mxs::device_info(&sms, &status);
     if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MXS_BF16)
-        launch_quantize<__nv_bfloat16>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st);
-    else if (dtype == MXS_F16)
-        launch_quantize<__half>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st);
-    else
-        launch_quantize<float>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st);
-    return cudaGetLastError() == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+    const cudaError_t e =
+        dtype == MXS_BF16  ? launch_quantize<__nv_bfloat16>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st)
+        : dtype == MXS_F16 ? launch_quantize<__half>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st)
+                           : launch_quantize<float>(d_x, ld_x, rows, cols, block_rows, d_q, ld_q, d_scale, st);
+    return e == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
 }
 
 int mxs_matmul_fp8_workspace_size(const void* d_a, int64_t ld_a, const void* d_b, int64_t ld_b, int64_t rows,
                                   int64_t n, int64_t k, size_t* bytes) {
     if (!bytes || rows < 0 || n <= 0 || k <= 0 || ld_a < k || ld_b < k || rows > LIMIT || n > LIMIT || k > LIMIT)
         return MXS_ERR_INVALID;
-    (void)d_a;
-    (void)d_b;
-    *bytes = 0;
+    *bytes = copies(nullptr, d_a, ld_a, d_b, ld_b, rows, n, k).bytes;
     return MXS_OK;
 }
 
@@ -195,23 +404,31 @@ int mxs_matmul_fp8(const void* d_a, int64_t ld_a, const float* d_a_scale, const 
         return MXS_ERR_INVALID;
     if (rows == 0) return MXS_OK;
     if (!d_a || !d_a_scale || !d_b || !d_b_scale || !d_out) return MXS_ERR_INVALID;
-    (void)d_workspace;
-    (void)workspace_bytes;
     int sms = 0;
     uint32_t* status = nullptr;
     int rc = mxs::device_info(&sms, &status);
     if (rc) return rc;
+    const Copies cp = copies(d_workspace, d_a, ld_a, d_b, ld_b, rows, n, k);
+    if (!mxs::workspace_ok(d_workspace, workspace_bytes, cp.bytes)) return MXS_ERR_WORKSPACE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    Mat p{static_cast<const uint8_t*>(d_a), static_cast<const uint8_t*>(d_b), ld_a, ld_b, d_a_scale, d_b_scale,
-          (int)rows, (int)n, (int)k, (int)ceil_div(k, BLK), d_out, ld_out};
-    const dim3 grid((unsigned)ceil_div(n, TN), (unsigned)ceil_div(rows, TM));
-    if (out_dtype == MXS_F32)
-        matmul_kernel<float><<<grid, 256, 0, st>>>(p);
-    else if (out_dtype == MXS_BF16)
-        matmul_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-    else
-        matmul_kernel<__half><<<grid, 256, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+    const int64_t ldk = round_up(k, 16);
+    if (cp.a) {
+        if (mxs::copy_rows(d_a, ld_a, cp.a, ldk, rows, k, sms, st) != cudaSuccess) return MXS_ERR_CUDA;
+        d_a = cp.a, ld_a = ldk;
+    }
+    if (cp.b) {
+        if (mxs::copy_rows(d_b, ld_b, cp.b, ldk, n, k, sms, st) != cudaSuccess) return MXS_ERR_CUDA;
+        d_b = cp.b, ld_b = ldk;
+    }
+    const bool pair = rows > 128;
+    auto go = [&](auto tag) {
+        using O = decltype(tag);
+        return pair ? launch_matmul<2, O>(d_a, ld_a, d_a_scale, d_b, ld_b, d_b_scale, rows, n, k, d_out, ld_out, sms,
+                                          status, st)
+                    : launch_matmul<1, O>(d_a, ld_a, d_a_scale, d_b, ld_b, d_b_scale, rows, n, k, d_out, ld_out, sms,
+                                          status, st);
+    };
+    return out_dtype == MXS_F32 ? go(0.0f) : out_dtype == MXS_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
 int mxs_sample_from_hidden_fp8_workspace_size(const void* d_weight_q, int64_t ld_weight, int64_t rows, int64_t d_model,

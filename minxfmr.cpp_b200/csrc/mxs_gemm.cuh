@@ -226,7 +226,8 @@ struct Ctx {
 //   load(t, kb, sa, sb, bar, ctx)
 //   zero(t, row, half, ctx)                                    the epilogue of a tile without blocks
 //   epilogue(t, tmem, row, half, ctx)                          !PROMOTE
-//   Acc, begin(...), join(...), finish(...)                    PROMOTE
+//   group(), Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulator is
+//                          read back and joined in registers after each `group` blocks
 template <typename Op>
 __device__ __forceinline__ void run(const Op& op) {
     constexpr int CG = Op::CG;
@@ -300,8 +301,10 @@ __device__ __forceinline__ void run(const Op& op) {
                 // MN-major: 64-wide slabs of 64 k rows (8192 bytes), 8-k groups 1024 bytes
                 // apart, a step of 16 k rows is 2048 bytes.
                 const uint64_t step_a = (amn ? 2048 : 32) >> 4, step_b = (bmn ? 2048 : 32) >> 4;
+                const int group = op.group() < t.kn ? op.group() : t.kn;
+                int in = 0;  // block of its group
                 for (int kb = 0; kb < t.kn; ++kb) {
-                    if (Op::PROMOTE || kb == 0) {
+                    if (in == 0) {
                         if (!wait(&ring->tempty[buf], tph ^ 1, ring)) { ok = false; break; }
                         fence_after();
                     }
@@ -312,13 +315,14 @@ __device__ __forceinline__ void run(const Op& op) {
                     uint64_t db = smem_desc(sa + A_BYTES, bmn ? 8192 : 16, 1024);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        mma<CG, Op::F8>(tmem + buf * 256, da, db, idesc, k > 0 || (!Op::PROMOTE && kb > 0));
+                        mma<CG, Op::F8>(tmem + buf * 256, da, db, idesc, k > 0 || in > 0);
                         da += step_a;
                         db += step_b;
                     }
                     commit<CG>(&ring->empty[s]);
                     if (++s == G::STAGES) s = 0, ph ^= 1;
-                    if (Op::PROMOTE || kb == t.kn - 1) {
+                    if (++in == group || kb == t.kn - 1) {
+                        in = 0;
                         commit<CG>(&ring->tfull[buf]);
                         if (++buf == 2) buf = 0, tph ^= 1;
                     }
@@ -344,7 +348,7 @@ __device__ __forceinline__ void run(const Op& op) {
             if constexpr (Op::PROMOTE) {
                 typename Op::Acc acc;
                 op.begin(acc, t, row, half, ctx);
-                for (int kb = 0; kb < t.kn; ++kb) {
+                for (int kb = 0; kb < t.kn; kb += op.group()) {
                     op.prepare(acc, t, t.k0 + kb, row, half, ctx);
                     ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                     if (!ok) break;
