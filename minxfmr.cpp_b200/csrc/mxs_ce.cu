@@ -244,17 +244,20 @@ struct ScoreOp : LogitTiles<CG_> {
         for (int i = 0; i < 128; ++i) a.v[i / 32][i % 32] = 0.0f;
     }
     __device__ void prepare(Acc&, const Tile&, int, int, int, const Ctx&) const {}
-    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
-        if (((t.m0 + row) & ~31) >= x.kept) return;  // no row of this warp
+    template <typename Release>
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx& x, Release release) const {
+        if (((t.m0 + row) & ~31) < x.kept) {  // a row of this warp
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = half * 32 + i * 64;
-            if (c0 >= t.n) break;
-            float v[32];
-            mxs::gemm::tmem_ld32(tmem + c0, v);
+            for (int i = 0; i < 4; i += 2) {
+                const int c0 = half * 32 + i * 64;
+                if (c0 >= t.n) break;
+                float v[32], w[32];
+                mxs::gemm::tmem_ld32x2(tmem + c0, tmem + (c0 + 64 < t.n ? c0 + 64 : c0), v, w);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a.v[i][j] += v[j];
+                for (int j = 0; j < 32; ++j) a.v[i][j] += v[j], a.v[i + 1][j] += w[j];
+            }
         }
+        release();
     }
     __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx& x) const {
         const int r = t.m0 + row;
@@ -353,7 +356,7 @@ struct GradLogitsOp : LogitTiles<CG_> {
         const int cols = live ? this->vocab - t.n0 : 0;
         T* out = g + (int64_t)r * ldg + t.n0;
         for (int c0 = half * 32; c0 < t.n; c0 += 64) {
-            float v[32];
+            float v[32] = {};
             if (any) {
                 mxs::gemm::tmem_ld32(tmem + c0, v);
 #pragma unroll

@@ -3,6 +3,7 @@
 // (mxs_quantize_fp8, mxs_matmul_fp8, mxs_sample_from_hidden_fp8).
 #include <algorithm>
 #include <cfloat>
+#include <cstring>
 
 #include <cuda_fp8.h>
 
@@ -26,17 +27,21 @@ __device__ __forceinline__ float block_scale(float top) {
     return top > 0.0f ? fmaxf(top / FP8_MAX, 1.17549435e-38f) : 1.0f;
 }
 
-// Eight values of a row, as 16-byte loads where they are aligned and whole.
-__device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], const __nv_bfloat16*) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight values of a row as they lie in memory.
+template <typename T>
+struct Raw {
+    uint4 u[sizeof(T) / 2];
+};
+__device__ __forceinline__ void values(const Raw<__nv_bfloat16>& x, float (&v)[8]) {
+    const uint32_t w[4] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(w[i] << 16);
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], const __half*) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void values(const Raw<__half>& x, float (&v)[8]) {
+    const uint32_t w[4] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -44,44 +49,33 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8], const __ha
         v[2 * i + 1] = f.y;
     }
 }
+__device__ __forceinline__ void values(const Raw<float>& x, float (&v)[8]) {
+    const uint32_t w[8] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w, x.u[1].x, x.u[1].y, x.u[1].z, x.u[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+// 16-byte loads where the eight are aligned and inside the row; zeros outside.
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, int n, bool vec, float (&v)[8]) {
+__device__ __forceinline__ Raw<T> load8(const T* x, int n, bool vec) {
+    Raw<T> r;
     if (vec && n >= 8) {
-        unpack(*reinterpret_cast<const uint4*>(x), v, x);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(x)[i];
     } else {
+        T t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(x[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) t[i] = i < n ? x[i] : mxs::from_f32<T>(0.0f);
+        memcpy(&r, t, sizeof r);
     }
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* x, int n, bool vec, float (&v)[8]) {
-    if (vec && n >= 8) {
-        const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? x[i] : 0.0f;
-    }
-}
-
-// The largest magnitude: NaN does not count; `all` keeps infinities in.
-__device__ __forceinline__ float top8(const float (&v)[8], bool all) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i]);
-        if (all || a <= FLT_MAX) m = fmaxf(m, a);
-    }
-    return m;
+    return r;
 }
 
 // x / s rounded to nearest, from r = 1 / s rounded to nearest: Markstein's
 // theorem (IBM J. Res. Dev. 34, 1990) makes q + r (x - q s) the correctly rounded
-// quotient for q = x r, as long as the remainder is exact. It is for s >= 2^-90
-// and quotients of at least 2^-11; smaller ones round to zero in 8 bits either
-// way. Smaller scales (`slow`) divide.
-__device__ __forceinline__ float quotient(float x, float s, float r, bool slow) {
-    if (slow) return x / s;
+// quotient for q = x r, as long as the remainder is exact. It is for finite x,
+// s >= 2^-90 and quotients of at least 2^-11; smaller ones round to zero in 8
+// bits either way.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
     const float q = x * r;
     return fmaf(fmaf(-q, s, x), r, q);
 }
@@ -90,18 +84,14 @@ __device__ __forceinline__ uint32_t quad(const float* y) {
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
-__device__ __forceinline__ void store8(uint8_t* q, int n, bool vec, const float (&v)[8], float s, float r, bool slow) {
-    float y[8];
+// The other blocks (a scale below 2^-90, or an infinity): one division each.
+template <typename T>
+__device__ __noinline__ uint2 divide8(const Raw<T> x, float s) {
+    float v[8];
+    values(x, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = quotient(v[i], s, r, slow);
-    const uint2 w = make_uint2(quad(y), quad(y + 4));
-    if (vec && n >= 8) {
-        *reinterpret_cast<uint2*>(q) = w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) q[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-    }
+    for (int i = 0; i < 8; ++i) v[i] = v[i] / s;
+    return make_uint2(quad(v), quad(v + 4));
 }
 
 // Bound by memory: each value is read once and kept in registers between its
@@ -109,73 +99,92 @@ __device__ __forceinline__ void store8(uint8_t* q, int n, bool vec, const float 
 // 128, a warp two neighbouring ones, twice. ROWS_OF = 128: a CTA of 256 threads
 // holds a block, sixteen lanes a row, eight rows each.
 template <typename T, int ROWS_OF>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols, uint8_t* q,
+__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, int rows, int cols, uint8_t* q,
                                                        int64_t ldq, float* scale, bool vec_in, bool vec_out) {
     constexpr int HELD = ROWS_OF == 1 ? 2 : 8;
     const int tid = threadIdx.x, lane = tid & 31, sub = tid & 15;
-    const int64_t bc = ceil_div(cols, BLK);
-    int64_t row[HELD], col[HELD];
+    const int bc = (cols + BLK - 1) / BLK;
+    int row0, col0;  // of the first eight; the others follow 256 columns or 16 rows on
     if (ROWS_OF == 1) {
-        const int64_t per_row = ceil_div(bc, 4);
-        const int64_t task = (int64_t)blockIdx.x * 8 + (tid >> 5);
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            row[i] = task / per_row;
-            col[i] = (task % per_row) * (4 * BLK) + i * (2 * BLK) + lane * 8;
-        }
+        const uint32_t per_row = (bc + 3) / 4, task = blockIdx.x * 8 + (tid >> 5);
+        row0 = task / per_row;
+        col0 = (task % per_row) * (4 * BLK) + lane * 8;
     } else {
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            row[i] = (int64_t)(blockIdx.x / bc) * BLK + i * 16 + (tid >> 4);
-            col[i] = (int64_t)(blockIdx.x % bc) * BLK + sub * 8;
-        }
+        row0 = (blockIdx.x / bc) * BLK + (tid >> 4);
+        col0 = (blockIdx.x % bc) * BLK + sub * 8;
     }
-    float v[HELD][8];
-    int n[HELD];
+    constexpr int DR = ROWS_OF == 1 ? 0 : 16, DC = ROWS_OF == 1 ? 2 * BLK : 0;
+    auto inside = [&](int i) { return row0 + i * DR < rows ? min(8, cols - col0 - i * DC) : 0; };  // may be negative
+    Raw<T> v[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        n[i] = row[i] < rows ? (int)min((int64_t)8, cols - col[i]) : 0;  // may be negative: nothing
-        load8(x + (n[i] > 0 ? row[i] * ldx + col[i] : 0), n[i], vec_in, v[i]);
+        const int n = inside(i);
+        v[i] = load8(n > 0 ? x + (int64_t)(row0 + i * DR) * ldx + col0 + i * DC : x, n, vec_in);
     }
-    __shared__ float s_top[8];
-    float s[HELD];
+    constexpr int TOPS = ROWS_OF == 1 ? HELD : 1;
+    __shared__ float s_top[2][8];
+    float top[TOPS];
+    bool inf = false;
     for (int pass = 0; pass < 2; ++pass) {  // the second pass leaves infinities out, where there are any
-        float top = 0.0f;
-        bool inf = false;
+        bool more = false;
+#pragma unroll
+        for (int i = 0; i < TOPS; ++i) top[i] = 0.0f;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const float mine = top8(v[i], pass == 0);
-            top = ROWS_OF == 1 ? mine : fmaxf(top, mine);
-            if (ROWS_OF == 1 || i == HELD - 1) {
+            float f[8];
+            values(v[i], f);
+            float m = top[i % TOPS];
 #pragma unroll
-                for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (ROWS_OF != 1) {
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    if (lane == 0) s_top[tid >> 5] = top;
-                    __syncthreads();
-#pragma unroll
-                    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
-                    __syncthreads();
-                }
-                inf |= top > FLT_MAX;
-                s[i] = top;
+            for (int j = 0; j < 8; ++j) {  // a NaN is not a maximum
+                const float a = fabsf(f[j]);
+                m = fmaxf(m, pass == 0 || a <= FLT_MAX ? a : 0.0f);
             }
+            top[i % TOPS] = m;
         }
-        // ROWS_OF 1: any block of the warp; 128: the same for the whole CTA
-        if (!__any_sync(0xffffffffu, inf)) break;
+#pragma unroll
+        for (int i = 0; i < TOPS; ++i) {
+#pragma unroll
+            for (int o = 8; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+            if (ROWS_OF != 1) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+                if (lane == 0) s_top[pass][tid >> 5] = top[i];
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < 8; ++w) top[i] = fmaxf(top[i], s_top[pass][w]);
+            }
+            more |= top[i] > FLT_MAX;
+        }
+        if (!__any_sync(0xffffffffu, more)) break;  // ROWS_OF 128: the whole CTA agrees
+        inf = true;
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const float sc = block_scale(s[ROWS_OF == 1 ? i : HELD - 1]);
-        const float r = 1.0f / sc;
-        // 2^-90; an infinity would spoil its own remainder
-        const bool slow = sc < 8.0779357e-28f || top8(v[i], true) > FLT_MAX;
-        if (n[i] > 0) {
-            store8(q + row[i] * ldq + col[i], n[i], vec_out, v[i], sc, r, slow);
-            if (ROWS_OF == 1 && sub == 0) scale[row[i] * bc + col[i] / BLK] = sc;
+        const int n = inside(i);
+        if (n <= 0) continue;
+        const int row = row0 + i * DR, col = col0 + i * DC;
+        const float s = block_scale(top[i % TOPS]);
+        const float r = 1.0f / s;
+        uint2 w;
+        if (inf || s < 8.0779357e-28f) {  // 2^-90
+            w = divide8(v[i], s);
+        } else {
+            float y[8];
+            values(v[i], y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = quotient(y[j], s, r);
+            w = make_uint2(quad(y), quad(y + 4));
         }
-        if (ROWS_OF != 1 && i == 0 && tid == 0) scale[blockIdx.x] = sc;
+        uint8_t* to = q + (int64_t)row * ldq + col;
+        if (vec_out && n >= 8) {
+            *reinterpret_cast<uint2*>(to) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) to[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+        }
+        if (ROWS_OF == 1 && sub == 0) scale[(int64_t)row * bc + col / BLK] = s;
     }
+    if (ROWS_OF != 1 && tid == 0) scale[blockIdx.x] = block_scale(top[0]);
 }
 
 template <typename T>
@@ -193,11 +202,11 @@ cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
         const int64_t n = std::min(most, rows - r);
         float* sc = scale + r / br * bc;
         if (br == 1)
-            quantize_kernel<T, 1><<<(unsigned)ceil_div(n * per, 8), 256, 0, st>>>(xt + r * ldx, ldx, n, cols,
-                                                                                 qt + r * ldq, ldq, sc, vin, vout);
+            quantize_kernel<T, 1><<<(unsigned)ceil_div(n * per, 8), 256, 0, st>>>(
+                xt + r * ldx, ldx, (int)n, (int)cols, qt + r * ldq, ldq, sc, vin, vout);
         else
             quantize_kernel<T, 128><<<(unsigned)(ceil_div(n, BLK) * per), 256, 0, st>>>(
-                xt + r * ldx, ldx, n, cols, qt + r * ldq, ldq, sc, vin, vout);
+                xt + r * ldx, ldx, (int)n, (int)cols, qt + r * ldq, ldq, sc, vin, vout);
     }
     return cudaGetLastError();
 }
@@ -268,16 +277,28 @@ struct MatmulOp {
         for (int i = 0; i < 4; ++i) a.now[i] = a.row_next * a.next[i];
         if (k + 1 < kb) fetch(a, t, k + 1, row, half);
     }
-    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx&) const {
-        if (((t.m0 + row) & ~31) >= rows) return;  // no row of this warp
+    template <typename Release>
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx&, Release release) const {
+        if (((t.m0 + row) & ~31) >= rows) {  // no row of this warp
+            release();
+            return;
+        }
+        float v[32], w[32];
+        const int c0 = half * 32;
+        mxs::gemm::tmem_ld32x2(tmem + c0, tmem + (c0 + 64 < t.n ? c0 + 64 : c0), v, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = half * 32 + i * 64;
-            if (c0 >= t.n) break;
-            float v[32];
-            mxs::gemm::tmem_ld32(tmem + c0, v);
+        for (int j = 0; j < 32; ++j) {
+            a.v[0][j] = fmaf(v[j], a.now[0], a.v[0][j]);
+            a.v[1][j] = fmaf(w[j], a.now[1], a.v[1][j]);
+        }
+        if (c0 + 128 < t.n) mxs::gemm::tmem_ld32x2(tmem + c0 + 128, tmem + (c0 + 192 < t.n ? c0 + 192 : c0), v, w);
+        release();
+        if (c0 + 128 < t.n) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(v[j], a.now[i], a.v[i][j]);
+            for (int j = 0; j < 32; ++j) {
+                a.v[2][j] = fmaf(v[j], a.now[2], a.v[2][j]);
+                a.v[3][j] = fmaf(w[j], a.now[3], a.v[3][j]);
+            }
         }
     }
     __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx&) const {

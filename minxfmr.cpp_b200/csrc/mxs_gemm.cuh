@@ -3,7 +3,10 @@
 //
 //   warp 0      loads operand tiles (TMA, 128-byte swizzle) into a ring of stages
 //   warp 1      issues tcgen05.mma (one thread), accumulators in TMEM
-//   warps 2..9  read accumulators back (tcgen05.ld) and do the Op's epilogue
+//   warps 4..11 read accumulators back (tcgen05.ld) and do the Op's epilogue
+//
+// Warps 0..3 give up registers for the epilogue's (setmaxnreg): 384 threads x 168
+// at launch = 128 x 56 + 256 x 224. The epilogue holds up to 128 sums a thread.
 //
 // A tile is 128 rows per CTA by up to 256 columns. With CG = 2 a pair of CTAs
 // works on one 256-row tile: each loads its 128 rows of A and half of B's
@@ -33,7 +36,8 @@
 namespace mxs {
 namespace gemm {
 
-constexpr int THREADS = 320;
+constexpr int THREADS = 384;
+constexpr int EPI_WARP0 = 4;
 constexpr int EPI_WARPS = 8;
 constexpr int A_BYTES = 128 * 128;
 constexpr int ROW = 128;  // bytes of a stage row (one swizzle row)
@@ -153,17 +157,41 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
         " tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr)
         : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Twice 32 columns with one wait.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t addr0, uint32_t addr1, float (&v)[32], float (&w)[32]) {
+    uint32_t r[32], q[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
+        " tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, "
+        "%44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, "
+        "[%65];\n"
+        " tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]),
+          "=r"(q[15]), "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]),
+          "=r"(q[22]), "=r"(q[23]), "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]),
+          "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+        : "r"(addr0), "r"(addr1)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]), w[i] = __uint_as_float(q[i]);
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: start address, leading and
@@ -182,18 +210,14 @@ __device__ __forceinline__ uint32_t instr_desc(int format, bool a_mn, bool b_mn,
 
 // --- waits -------------------------------------------------------------------
 
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return done != 0;
-}
-// False (and the CTA is dead) when the limit ran out or another role gave up.
+// False (and the CTA is dead) when the limit ran out or another role gave up. The
+// clock is read after 32 polls only: it is a slow read next to a wait of a few
+// hundred clocks, and there are several of those for every block of the ring.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ring* ring) {
-    if (try_wait_cluster(bar, parity)) return true;
+    for (int i = 0; i < 32; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
-    while (!try_wait_cluster(bar, parity)) {
+    while (!mbar_try_wait(bar, parity)) {
         if (*(volatile int*)&ring->dead) return false;
         if (globaltimer_ns() - t0 > 1000000000ull) {
             *(volatile int*)&ring->dead = 1;
@@ -202,8 +226,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ring* ring)
     }
     return true;
 }
+// An accumulator's readers tell the MMA thread of the pair. What they hand over
+// is TMEM, ordered by the tcgen05 fences; no memory is published, so the arrival
+// is relaxed (a release for the cluster waits for every load and store in flight:
+// 1000 to 2000 clocks for each block of the 8-bit product).
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // What an Op needs to know of where it runs.
@@ -266,8 +294,9 @@ __device__ __forceinline__ void run(const Op& op) {
     ctx.kept = op.kept();
 
     Tile t;
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < EPI_WARP0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && lane == 0) {
             uint32_t s = 0, ph = 0;
             int64_t issued = 0;
             bool ok = true;
@@ -290,8 +319,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     mbar_wait_bounded(&ring->full[j % G::STAGES], (uint32_t)(j / G::STAGES) & 1);
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0 && ctx.rank == 0) {
+        if (warp == 1 && lane == 0 && ctx.rank == 0) {
             uint32_t s = 0, ph = 0, buf = 0, tph = 0;
             bool ok = true;
             for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
@@ -334,7 +362,8 @@ __device__ __forceinline__ void run(const Op& op) {
             }
         }
     } else {
-        const int quad = warp & 3, half = (warp - 2) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quad = warp & 3, half = (warp - EPI_WARP0) >> 2;
         const int row = (int)ctx.rank * 128 + quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t te0 = CG == 2 ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
@@ -353,10 +382,12 @@ __device__ __forceinline__ void run(const Op& op) {
                     ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                     if (!ok) break;
                     fence_after();
-                    op.join(acc, t, tmem + buf * 256 + lanes, row, half, ctx);
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_remote(te0 + buf * 8);
+                    // the accumulator goes back to the MMAs as soon as it has been read
+                    op.join(acc, t, tmem + buf * 256 + lanes, row, half, ctx, [&] {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_remote(te0 + buf * 8);
+                    });
                     if (++buf == 2) buf = 0, tph ^= 1;
                 }
                 if (ok) op.finish(acc, t, row, half, ctx);

@@ -6,16 +6,41 @@ As in the rest of the package torch only carries memory and streams. Outputs and
 scratch are torch tensors of the call's stream (`stream`, or the current one), so
 calls on different streams share none.
 """
+import contextlib
 import ctypes
 
 import torch
 
-from . import _check, _need_cuda, _ptr, _stream, k_use, load
+from . import _check, _need_cuda, k_use, load
 
 BF16, F16, F32 = 0, 1, 2
 _CODES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 FP8 = torch.float8_e4m3fn
 BLOCK = 128
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(stream):
+    return (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+@contextlib.contextmanager
+def _elsewhere(dev, stream):
+    with torch.cuda.device(dev), torch.cuda.stream(stream):
+        yield
+
+
+def _on(dev, stream):
+    """The device and stream of a call made current, where they are not."""
+    if stream is None and dev.index == torch.cuda.current_device():
+        return _HERE
+    return _elsewhere(dev, stream)
 
 
 def _code(t, name, allowed):
@@ -74,7 +99,7 @@ def ce_from_hidden(hidden, weight, targets, temperature=1.0, stream=None):
     log-probability."""
     dt, rows, d, vocab, ldh, ldw, tb = _ce_operands(hidden, weight, targets, temperature)
     dev = hidden.device
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
+    with _on(dev, stream):
         loss = torch.empty(rows, dtype=torch.float32, device=dev)
         lse = torch.empty(rows, dtype=torch.float32, device=dev)
         ws = _scratch("mxs_ce_workspace_size", (_ptr(weight), ldw, rows, d, vocab, 0), dev)
@@ -95,7 +120,7 @@ def ce_from_hidden_backward(hidden, weight, targets, lse, grad_loss, temperature
     _same_device(dev, lse=lse, grad_loss=grad_loss)
     _vector(lse, rows, "lse", (torch.float32,))
     _vector(grad_loss, rows, "grad_loss", (torch.float32,))
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
+    with _on(dev, stream):
         gh = torch.empty((rows, d), dtype=hidden.dtype, device=dev) if need_hidden else None
         gw = torch.empty((vocab, d), dtype=hidden.dtype, device=dev) if need_weight else None
         ws = _scratch("mxs_ce_workspace_size", (_ptr(weight), ldw, rows, d, vocab, 1), dev)
@@ -143,7 +168,7 @@ def quantize_fp8(x, block_rows, stream=None):
         raise ValueError("x must have columns")
     dev = x.device
     ldq = -(-cols // 16) * 16
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
+    with _on(dev, stream):
         q = torch.empty((rows, ldq), dtype=FP8, device=dev)[:, :cols]
         scale = torch.empty((-(-rows // block_rows), -(-cols // BLOCK)), dtype=torch.float32, device=dev)
         rc = load().mxs_quantize_fp8(_ptr(x), ldx, dt, rows, cols, block_rows, _ptr(q), ldq, _ptr(scale),
@@ -172,7 +197,7 @@ def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.float32, out=None, stream
     _scale(b_scale, (-(-n // BLOCK), kb), "b_scale")
     dev = a.device
     _same_device(dev, a_scale=a_scale, b=b, b_scale=b_scale, out=out)
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
+    with _on(dev, stream):
         if out is None:
             if out_dtype not in _CODES:
                 raise ValueError("out_dtype must be float32, bfloat16 or float16")
@@ -207,7 +232,7 @@ def sample_from_hidden_fp8(hidden, weight_q, weight_scale, temperature, top_k, u
         raise ValueError(f"logits_out must be [{rows}, {vocab}] float32")
     ldl = 0 if logits_out is None else _matrix(logits_out, "logits_out")
     k = k_use(int(top_k), vocab)
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
+    with _on(dev, stream):
         nxt = torch.empty(rows, dtype=torch.int32, device=dev)
         idx = torch.empty((rows, k), dtype=torch.int32, device=dev) if return_topk else None
         prob = torch.empty((rows, k), dtype=torch.float64, device=dev) if return_topk else None
