@@ -78,6 +78,12 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// True in one thread of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -296,30 +302,38 @@ __device__ __forceinline__ void run(const Op& op) {
     Tile t;
     if (warp < EPI_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0 && lane == 0) {
+        // Both roles run as whole warps with one elected thread at the loads and MMAs:
+        // addresses and descriptors then stay in uniform registers, which those
+        // instructions want (from a single-thread branch a block's four MMAs took
+        // 670 clocks to issue, more than the 512 that they run).
+        if (warp == 0) {
             uint32_t s = 0, ph = 0;
             int64_t issued = 0;
             bool ok = true;
-            for (int i = 0; ok && op.tile(i, ctx, t); ++i)
+            for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
+                const uint32_t bytes = CG * op.bytes(t);
                 for (int kb = 0; kb < t.kn; ++kb) {
-                    if (!wait(&ring->empty[s], ph ^ 1, ring)) { ok = false; break; }
-                    if (op.drop >= 0 && blockIdx.x == 0 && issued >= op.drop) { ok = false; break; }
-                    uint32_t bar = smem_u32(&ring->full[s]);
-                    if (ctx.rank == 0) mbar_arrive_expect_tx(&ring->full[s], CG * op.bytes(t));
-                    if (CG == 2) bar = map_to_rank(bar, 0);
-                    const uint32_t sa = stages + s * G::STAGE;
-                    op.load(t, t.k0 + kb, sa, sa + A_BYTES, bar, ctx);
+                    ok = wait(&ring->empty[s], ph ^ 1, ring) && !(op.drop >= 0 && blockIdx.x == 0 && issued >= op.drop);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    if (elect()) {
+                        uint32_t bar = smem_u32(&ring->full[s]);
+                        if (ctx.rank == 0) mbar_arrive_expect_tx(&ring->full[s], bytes);
+                        if (CG == 2) bar = map_to_rank(bar, 0);
+                        const uint32_t sa = stages + s * G::STAGE;
+                        op.load(t, t.k0 + kb, sa, sa + A_BYTES, bar, ctx);
+                    }
+                    __syncwarp();
                     ++issued;
                     if (++s == G::STAGES) s = 0, ph ^= 1;
                 }
+            }
             // gave up: the copies still in flight (at most one per stage) land before the CTA ends
             if (!ok && ctx.rank == 0) {
                 const int64_t n = issued < G::STAGES ? issued : (int64_t)G::STAGES;
                 for (int64_t j = issued - n; j < issued; ++j)
                     mbar_wait_bounded(&ring->full[j % G::STAGES], (uint32_t)(j / G::STAGES) & 1);
             }
-        }
-        if (warp == 1 && lane == 0 && ctx.rank == 0) {
+        } else if (warp == 1 && ctx.rank == 0) {
             uint32_t s = 0, ph = 0, buf = 0, tph = 0;
             bool ok = true;
             for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
@@ -329,35 +343,36 @@ __device__ __forceinline__ void run(const Op& op) {
                 // MN-major: 64-wide slabs of 64 k rows (8192 bytes), 8-k groups 1024 bytes
                 // apart, a step of 16 k rows is 2048 bytes.
                 const uint64_t step_a = (amn ? 2048 : 32) >> 4, step_b = (bmn ? 2048 : 32) >> 4;
+                const uint64_t da0 = smem_desc(stages, amn ? 8192 : 16, 1024);
+                const uint64_t db0 = smem_desc(stages + A_BYTES, bmn ? 8192 : 16, 1024);
                 const int group = op.group() < t.kn ? op.group() : t.kn;
                 int in = 0;  // block of its group
                 for (int kb = 0; kb < t.kn; ++kb) {
-                    if (in == 0) {
-                        if (!wait(&ring->tempty[buf], tph ^ 1, ring)) { ok = false; break; }
-                        fence_after();
-                    }
-                    if (!wait(&ring->full[s], ph, ring)) { ok = false; break; }
+                    ok = (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring)) && wait(&ring->full[s], ph, ring);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     fence_after();
-                    const uint32_t sa = stages + s * G::STAGE;
-                    uint64_t da = smem_desc(sa, amn ? 8192 : 16, 1024);
-                    uint64_t db = smem_desc(sa + A_BYTES, bmn ? 8192 : 16, 1024);
+                    const bool last = in + 1 == group || kb == t.kn - 1;
+                    if (elect()) {
+                        const uint64_t da = da0 + (uint64_t)(s * (G::STAGE >> 4)), db = db0 + (uint64_t)(s * (G::STAGE >> 4));
+                        const uint32_t d = tmem + buf * 256;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        mma<CG, Op::F8>(tmem + buf * 256, da, db, idesc, k > 0 || in > 0);
-                        da += step_a;
-                        db += step_b;
+                        for (int k = 0; k < 4; ++k)
+                            mma<CG, Op::F8>(d, da + k * step_a, db + k * step_b, idesc, k > 0 || in > 0);
+                        commit<CG>(&ring->empty[s]);
+                        if (last) commit<CG>(&ring->tfull[buf]);
                     }
-                    commit<CG>(&ring->empty[s]);
+                    __syncwarp();
+                    ++in;
                     if (++s == G::STAGES) s = 0, ph ^= 1;
-                    if (++in == group || kb == t.kn - 1) {
+                    if (last) {
                         in = 0;
-                        commit<CG>(&ring->tfull[buf]);
                         if (++buf == 2) buf = 0, tph ^= 1;
                     }
                 }
             }
             if (!ok) {  // MMAs in flight finish before TMEM is freed
-                commit<CG>(&ring->drain);
+                if (elect()) commit<CG>(&ring->drain);
+                __syncwarp();
                 mbar_wait_bounded(&ring->drain, 0);
             }
         }
