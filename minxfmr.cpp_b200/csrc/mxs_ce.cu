@@ -34,6 +34,7 @@ using mxs::Carve;
 using mxs::ceil_div;
 using mxs::round_up;
 using mxs::gemm::Ctx;
+using mxs::gemm::Lane;
 using mxs::gemm::Tile;
 
 constexpr int64_t MAX_DIM = INT32_MAX - 1024;
@@ -219,12 +220,13 @@ struct LogitTiles {
         mxs::gemm::tma_load<CG>(sa, &mh, kb * 64, t.m0 + (int)x.rank * 128, bar);
         mxs::gemm::tma_load<CG>(sb, &mw, kb * 64, v0 + t.n0 + (int)x.rank * (n / CG), bar);
     }
-    __device__ void zero(const Tile&, int, int, const Ctx&) const {}
+    __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
 };
 
-// Each thread holds half a tile's columns of one row: the largest y of the others
-// and sum 2^(y - largest). The exponentials run at 16 a clock and SM: 2048 clocks
-// for 128 x 256, under the 512 clocks of each 64 of d_model that the products take.
+// Each thread holds a quarter of a tile's columns of one row: the largest y of
+// the others and sum 2^(y - largest); the four of a row meet in shared memory. The
+// exponentials run at 16 a clock and SM: 2048 clocks for 128 x 256, against 512
+// clocks of MMA for each 64 of d_model.
 // The MMA's own fp32 sum rounds towards zero at every 16 products, which at
 // d_model 3584 leaves 2e-6 of the logits' size; joining the accumulator in
 // registers (round to nearest) every 1024 products keeps it below 1e-6 and costs
@@ -234,46 +236,50 @@ struct ScoreOp : LogitTiles<CG_> {
     static constexpr bool PROMOTE = true;
     __device__ int group() const { return 16; }
     struct Acc {
-        float v[4][32];
+        float v[2][32];
     };
-    float2* part;    // [tile * 2 + half][rows]
+    float2* part;    // [tile][rows]
     float* ytarget;  // [rows]
 
-    __device__ void begin(Acc& a, const Tile&, int, int, const Ctx&) const {
+    __device__ void begin(Acc& a, const Tile&, const Lane&, const Ctx&) const {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) a.v[i / 32][i % 32] = 0.0f;
+        for (int i = 0; i < 64; ++i) a.v[i / 32][i % 32] = 0.0f;
     }
-    __device__ void prepare(Acc&, const Tile&, int, int, int, const Ctx&) const {}
+    __device__ void prepare(Acc&, const Tile&, int, const Lane&, const Ctx&) const {}
     template <typename Release>
-    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx& x, Release release) const {
-        if (((t.m0 + row) & ~31) < x.kept) {  // a row of this warp
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x, Release release) const {
+        if (((t.m0 + me.row) & ~31) < x.kept) {  // a row of this warp
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const int c0 = half * 32 + i * 64;
-                if (c0 >= t.n) break;
-                float v[32], w[32];
-                mxs::gemm::tmem_ld32x2(tmem + c0, tmem + (c0 + 64 < t.n ? c0 + 64 : c0), v, w);
+            for (int i = 0; i < 2; ++i) {
+                const int c0 = me.grp * 32 + i * 128;
+                if (c0 < t.n) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) a.v[i][j] += v[j], a.v[i + 1][j] += w[j];
+                    for (int h = 0; h < 32; h += 16) {
+                        float v[16];
+                        mxs::gemm::tmem_ld16(tmem + c0 + h, v);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) a.v[i][h + j] += v[j];
+                    }
+                }
             }
         }
         release();
     }
-    __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx& x) const {
-        const int r = t.m0 + row;
-        if ((r & ~31) >= x.kept) return;
+    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx& x) const {
+        const int r = t.m0 + me.row;
+        if ((r & ~31) >= x.kept) return;  // the four warps of these rows agree
         const int hit = r < x.kept ? this->target[r] - t.n0 : -1;  // the target's column of this tile
         const int cols = min(t.n, this->vocab - t.n0);
         float m = -INFINITY, s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = half * 32 + i * 64;
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = me.grp * 32 + i * 128;
             if (c0 >= t.n) break;
             float(&v)[32] = a.v[i];
             if (hit >= c0 && hit < c0 + 32) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                    if (j == hit - c0) {
+                    if (mxs::gemm::is_column(hit - c0, j)) {
                         ytarget[r] = v[j] * this->c;
                         v[j] = -INFINITY;
                     }
@@ -294,7 +300,19 @@ struct ScoreOp : LogitTiles<CG_> {
             s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
             m = nm;
         }
-        if (r < x.kept) part[((int64_t)t.kind * 2 + half) * this->rows + r] = make_float2(m, s);
+        // two buffers: a warp is at most one tile ahead of the others of its rows
+        float2* mine = reinterpret_cast<float2*>(me.xpose) + (t.seq & 1) * 32 + me.lane;
+        *mine = make_float2(m, s);
+        asm volatile("bar.sync %0, 128;" ::"r"(me.quad + 1) : "memory");
+        if (me.grp != 0 || r >= x.kept) return;
+#pragma unroll
+        for (int g = 1; g < 4; ++g) {  // group g's warp is four places on
+            const float2 q = mine[g * 4 * (mxs::gemm::XPOSE / 8)];
+            const float nm = fmaxf(m, q.x), sub = nm == -INFINITY ? 0.0f : nm;
+            s = s * ex2(m - sub) + q.y * ex2(q.x - sub);
+            m = nm;
+        }
+        part[(int64_t)t.kind * this->rows + r] = make_float2(m, s);
     }
 };
 
@@ -346,33 +364,33 @@ struct GradLogitsOp : LogitTiles<CG_> {
     int ldg;
     float gscale;
 
-    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx& x) const {
-        const int r = t.m0 + row;
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x) const {
+        const int r = t.m0 + me.row;
         const bool live = r < x.kept;
-        const bool any = (r & ~31) < x.kept;
         const int hit = live ? this->target[r] - this->v0 - t.n0 : -1;
         const float l2 = live ? lse2[r] : 0.0f;
         const float gr = live ? ghat[r] * gscale : 0.0f;
-        const int cols = live ? this->vocab - t.n0 : 0;
-        T* out = g + (int64_t)r * ldg + t.n0;
-        for (int c0 = half * 32; c0 < t.n; c0 += 64) {
-            float v[32] = {};
-            if (any) {
-                mxs::gemm::tmem_ld32(tmem + c0, v);
+        const int cols = this->vocab - t.n0;
+        T* out = g + (int64_t)(r - me.lane) * ldg + t.n0;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->c, -l2)) * gr;
-                if (hit >= c0 && hit < c0 + 32) {
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = me.grp * 32 + i * 128;
+            if (c0 >= t.n || t.n0 + c0 >= ldg) break;
+            float v[32];
+            mxs::gemm::tmem_ld32(tmem + c0, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (j == hit - c0) v[j] -= gr;
-                }
-            }
-            if (!any || c0 + 32 > cols) {
+            for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->c, -l2)) * gr;
+            if (hit >= c0 && hit < c0 + 32) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                    if (c0 + j >= cols) v[j] = 0.0f;
+                    if (mxs::gemm::is_column(hit - c0, j)) v[j] -= gr;
             }
-            mxs::store32(out + c0, v, ldg - t.n0 - c0, true);
+            if (!live || c0 + 32 > cols) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (!live || c0 + j >= cols) v[j] = 0.0f;
+            }
+            mxs::gemm::store_rows<T, false>(out + c0, ldg, v, 32, 32, true, me);
         }
     }
 };
@@ -454,47 +472,41 @@ struct ProductOp {
         const int kr = t.kind >= 0 ? v0 + k : k;
         for (int j = 0; j < n / 128; ++j) mxs::gemm::tma_load<2>(sb + j * 8192, b, c + 64 * j, kr, bar);
     }
-    __device__ void epilogue(const Tile& t, uint32_t tmem, int row, int half, const Ctx&) const {
-        if (t.kind >= 0) {
-            float* a = acc + ((int64_t)t.kind * 256 + row) * 256;
-            for (int c0 = half * 32; c0 < n; c0 += 64) {
-                float v[32];
-                mxs::gemm::tmem_ld32(tmem + c0, v);
-                float4* p = reinterpret_cast<float4*>(a + c0);
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&) const {
+        const float s = t.kind >= 0 ? 1.0f : head->gmax * scale;
+        const int m = t.m0 + me.row - me.lane;  // first row of the warp
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float4 q = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                    if (!first) {
-                        const float4 o = p[j];
-                        q = make_float4(q.x + o.x, q.y + o.y, q.z + o.z, q.w + o.w);
-                    }
-                    p[j] = q;
-                }
-            }
-            return;
-        }
-        const float s = head->gmax * scale;
-        const int m = t.m0 + row;
-        T* out = dw + (int64_t)(v0 + m) * lddw + t.n0;
-        for (int c0 = half * 32; c0 < n; c0 += 64) {
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = me.grp * 32 + i * 128;
+            if (c0 >= n) break;
             float v[32];
             mxs::gemm::tmem_ld32(tmem + c0, v);
+            if (t.kind >= 0) {
+                float* a = acc + ((int64_t)t.kind * 256 + me.row - me.lane) * 256 + c0;
+                if (first)
+                    mxs::gemm::store_rows<float, false>(a, 256, v, 32, 32, true, me);
+                else
+                    mxs::gemm::store_rows<float, true>(a, 256, v, 32, 32, true, me);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= s;
-            if (m < width) mxs::store32(out + c0, v, d - t.n0 - c0, vec);
+                for (int j = 0; j < 32; ++j) v[j] *= s;
+                mxs::gemm::store_rows<T, false>(dw + (int64_t)(v0 + m) * lddw + t.n0 + c0, lddw, v, width - m,
+                                                d - t.n0 - c0, vec, me);
+            }
         }
     }
-    __device__ void zero(const Tile& t, int row, int half, const Ctx&) const {
+    __device__ void zero(const Tile& t, const Lane& me, const Ctx&) const {
         if (t.kind >= 0) {  // a split without columns
-            float* a = acc + ((int64_t)t.kind * 256 + row) * 256;
+            float* a = acc + ((int64_t)t.kind * 256 + me.row) * 256;
             if (first)
-                for (int c0 = half * 128; c0 < min(n, half * 128 + 128); ++c0) a[c0] = 0.0f;
+                for (int c0 = me.grp * 64; c0 < min(n, me.grp * 64 + 64); ++c0) a[c0] = 0.0f;
             return;
         }
-        const int m = t.m0 + row;
+        const int m = t.m0 + me.row;
         if (m >= width) return;
         T* out = dw + (int64_t)(v0 + m) * lddw + t.n0;
-        for (int c0 = half * 128; c0 < min(min(n, half * 128 + 128), d - t.n0); ++c0) out[c0] = mxs::from_f32<T>(0.0f);
+        for (int c0 = me.grp * 64; c0 < min(min(n, me.grp * 64 + 64), d - t.n0); ++c0)
+            out[c0] = mxs::from_f32<T>(0.0f);
     }
 };
 
@@ -558,7 +570,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     if (!backward) {
         pl.n = mxs::tile_width(ceil_div(rows, 128 * cg), vocab, sms / cg, 64, 32);
         pl.nt = (int)ceil_div(vocab, pl.n);
-        pl.part = c.take<float2>((size_t)pl.nt * 2 * rows);
+        pl.part = c.take<float2>((size_t)pl.nt * rows);
         pl.ytarget = c.take<float>(rows);
     } else {
         pl.lse2 = c.take<float>(rows);
@@ -659,7 +671,7 @@ int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss
     const int64_t tiles = ceil_div(a.rows, 128 * CG) * pl.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
     MXS_TRY(launch_dependent(score_join_kernel, (unsigned)ceil_div(a.rows, 8), 256, a.st, pl.part, pl.ytarget, pl.pos,
-                             (int)a.rows, pl.nt * 2, loss, lse));
+                             (int)a.rows, pl.nt, loss, lse));
     return MXS_OK;
 }
 

@@ -17,6 +17,7 @@ using mxs::Carve;
 using mxs::ceil_div;
 using mxs::round_up;
 using mxs::gemm::Ctx;
+using mxs::gemm::Lane;
 using mxs::gemm::Tile;
 using mxs::to_f32;
 
@@ -225,8 +226,8 @@ struct MatmulOp {
     static constexpr bool F8 = true, PROMOTE = true;
     __device__ int group() const { return 1; }
     struct Acc {
-        float v[4][32];
-        float row_next, next[4], now[4];  // scales of the next block and of this one
+        float v[2][32];
+        float row_next, next[2], now[2];  // scales of the next block and of this one
     };
     CUtensorMap ma, mb;
     int format;
@@ -257,59 +258,56 @@ struct MatmulOp {
         mxs::gemm::tma_load<CG>(s_a, &ma, k * BLK, t.m0 + (int)x.rank * 128, bar);
         mxs::gemm::tma_load<CG>(s_b, &mb, k * BLK, t.n0 + (int)x.rank * (n / CG), bar);
     }
-    __device__ void zero(const Tile&, int, int, const Ctx&) const {}
-    __device__ void fetch(Acc& a, const Tile& t, int k, int row, int half) const {
-        const float s = sa[(int64_t)min(rows - 1, t.m0 + row) * kb + k];
+    __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
+    __device__ void fetch(Acc& a, const Tile& t, int k, const Lane& me) const {
+        a.row_next = sa[(int64_t)min(rows - 1, t.m0 + me.row) * kb + k];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = min(cols - 1, t.n0 + half * 32 + i * 64);  // 32 columns lie in one block of 128
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = min(cols - 1, t.n0 + me.grp * 32 + i * 128);  // 32 columns lie in one block of 128
             a.next[i] = sb[(int64_t)(c0 / BLK) * kb + k];
         }
-        a.row_next = s;
     }
-    __device__ void begin(Acc& a, const Tile& t, int row, int half, const Ctx&) const {
+    __device__ void begin(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) a.v[i / 32][i % 32] = 0.0f;
-        fetch(a, t, 0, row, half);
+        for (int i = 0; i < 64; ++i) a.v[i / 32][i % 32] = 0.0f;
+        fetch(a, t, 0, me);
     }
-    __device__ void prepare(Acc& a, const Tile& t, int k, int row, int half, const Ctx&) const {
+    __device__ void prepare(Acc& a, const Tile& t, int k, const Lane& me, const Ctx&) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a.now[i] = a.row_next * a.next[i];
-        if (k + 1 < kb) fetch(a, t, k + 1, row, half);
+        for (int i = 0; i < 2; ++i) a.now[i] = a.row_next * a.next[i];
+        if (k + 1 < kb) fetch(a, t, k + 1, me);
     }
     template <typename Release>
-    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, int row, int half, const Ctx&, Release release) const {
-        if (((t.m0 + row) & ~31) >= rows) {  // no row of this warp
+    __device__ void join(Acc& a, const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, Release release) const {
+        const int c0 = me.grp * 32;
+        if (((t.m0 + me.row) & ~31) >= rows || c0 >= t.n) {  // no row or column of this warp
             release();
             return;
         }
-        float v[32], w[32];
-        const int c0 = half * 32;
-        mxs::gemm::tmem_ld32x2(tmem + c0, tmem + (c0 + 64 < t.n ? c0 + 64 : c0), v, w);
+        const int runs = c0 + 128 < t.n ? 2 : 1;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            a.v[0][j] = fmaf(v[j], a.now[0], a.v[0][j]);
-            a.v[1][j] = fmaf(w[j], a.now[1], a.v[1][j]);
-        }
-        if (c0 + 128 < t.n) mxs::gemm::tmem_ld32x2(tmem + c0 + 128, tmem + (c0 + 192 < t.n ? c0 + 192 : c0), v, w);
-        release();
-        if (c0 + 128 < t.n) {
+        for (int i = 0; i < 2; ++i) {
+            if (i >= runs) break;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                a.v[2][j] = fmaf(v[j], a.now[2], a.v[2][j]);
-                a.v[3][j] = fmaf(w[j], a.now[3], a.v[3][j]);
+            for (int h = 0; h < 32; h += 16) {
+                float v[16];
+                mxs::gemm::tmem_ld16(tmem + c0 + i * 128 + h, v);
+                if (h == 16 && i == runs - 1) release();
+#pragma unroll
+                for (int j = 0; j < 16; j += 2)
+                    mxs::gemm::fma2(a.v[i][h + j], a.v[i][h + j + 1], v[j], v[j + 1], a.now[i]);
             }
         }
     }
-    __device__ void finish(Acc& a, const Tile& t, int row, int half, const Ctx&) const {
-        const int r = t.m0 + row;
-        if (r >= rows) return;
-        O* o = out + (int64_t)r * ldo + t.n0;
+    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
+        const int r0 = t.m0 + me.row - me.lane;
+        if (r0 >= rows) return;
+        O* o = out + (int64_t)r0 * ldo + t.n0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = half * 32 + i * 64;
-            if (c0 >= t.n) break;
-            mxs::store32(o + c0, a.v[i], cols - t.n0 - c0, vec);
+        for (int i = 0; i < 2; ++i) {
+            const int c0 = me.grp * 32 + i * 128;
+            if (c0 < t.n)
+                mxs::gemm::store_rows<O, false>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
         }
     }
 };

@@ -3,10 +3,13 @@
 //
 //   warp 0      loads operand tiles (TMA, 128-byte swizzle) into a ring of stages
 //   warp 1      issues tcgen05.mma (one thread), accumulators in TMEM
-//   warps 4..11 read accumulators back (tcgen05.ld) and do the Op's epilogue
+//   warps 4..19 read accumulators back (tcgen05.ld) and do the Op's epilogue: four
+//               warps share the 32 rows that the hardware gives a warp's place, in
+//               four column groups of 32 (a thread has up to two runs of 32 columns)
 //
-// Warps 0..3 give up registers for the epilogue's (setmaxnreg): 384 threads x 168
-// at launch = 128 x 56 + 256 x 224. The epilogue holds up to 128 sums a thread.
+// Sixteen epilogue warps, not eight, because a read of an accumulator takes some
+// hundred clocks and only other warps can fill them. Warps 0..3 give up registers
+// for them (setmaxnreg): 640 threads x 96 at launch = 128 x 64 + 512 x 104.
 //
 // A tile is 128 rows per CTA by up to 256 columns. With CG = 2 a pair of CTAs
 // works on one 256-row tile: each loads its 128 rows of A and half of B's
@@ -32,13 +35,15 @@
 #include <cuda.h>
 
 #include "mxs_common.cuh"
+#include "mxs_head.cuh"
 
 namespace mxs {
 namespace gemm {
 
-constexpr int THREADS = 384;
+constexpr int THREADS = 640;
 constexpr int EPI_WARP0 = 4;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
+constexpr int XPOSE = 2048;  // bytes of shared memory for each epilogue warp's transposes
 constexpr int A_BYTES = 128 * 128;
 constexpr int ROW = 128;  // bytes of a stage row (one swizzle row)
 
@@ -47,7 +52,7 @@ struct Geo {
     static constexpr int B_BYTES = 256 / CG * ROW;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = 196608 / STAGE;  // 192 KB: 4 or 6
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 1024;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + EPI_WARPS * XPOSE + 512;
 };
 
 struct Tile {
@@ -55,6 +60,14 @@ struct Tile {
     int k0, kn;   // first k block and number of blocks
     int n;        // columns of the MMA
     int kind;     // Op's own
+    int seq;      // which of this unit's tiles
+};
+
+// An epilogue thread's place.
+struct Lane {
+    int lane, quad, grp;  // quad: which 32 rows of the CTA's 128; grp: which column group
+    int row;              // of the pair's tile
+    uint8_t* xpose;       // its warp's XPOSE bytes
 };
 
 struct Ring {
@@ -175,29 +188,78 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// Twice 32 columns with one wait.
-__device__ __forceinline__ void tmem_ld32x2(uint32_t addr0, uint32_t addr1, float (&v)[32], float (&w)[32]) {
-    uint32_t r[32], q[32];
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
-        " tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, "
-        "%44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, "
-        "[%65];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15},"
+        " [%16];\n"
         " tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
-          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]),
-          "=r"(q[15]), "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]),
-          "=r"(q[22]), "=r"(q[23]), "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]),
-          "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
-        : "r"(addr0), "r"(addr1)
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]), w[i] = __uint_as_float(q[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Whether the unrolled j is the value h, kept as a comparison (the compiler would
+// turn the run of them into an index, and the array into local memory).
+__device__ __forceinline__ bool is_column(int h, int j) {
+    int d = h - j;
+    asm("" : "+r"(d));
+    return d == 0;
+}
+
+// a * b + c on two pairs of floats.
+__device__ __forceinline__ void fma2(float& x, float& y, float a0, float a1, float b) {
+    asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %4};\n mov.b64 r, {%0, %1};\n"
+        " fma.rn.f32x2 r, p, q, r;\n mov.b64 {%0, %1}, r;\n}" : "+f"(x), "+f"(y) : "f"(a0), "f"(a1), "f"(b));
+}
+
+// A warp's 32 x 32 values (a row a thread) to row-major memory, through its
+// XPOSE bytes: a store from the threads' own rows touches 32 lines for 16 bytes
+// each, one from here 8 rows of 64 bytes. `out` is the place of row 0, column 0;
+// `rows` and `cols` say how many of the 32 exist; `vec` that rows start on 16-byte
+// boundaries. ADD adds to what is there.
+template <typename T, bool ADD>
+__device__ __forceinline__ void store_rows(T* out, int64_t ld, const float (&v)[32], int rows, int cols, bool vec,
+                                           const Lane& me) {
+    constexpr int EACH = 16 / sizeof(T);  // values of a 16-byte piece; a pass takes four pieces of a row
+    constexpr int W = 4 * EACH;
+    const int l = me.lane;
+#pragma unroll
+    for (int c0 = 0; c0 < 32; c0 += W) {
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            *reinterpret_cast<uint4*>(me.xpose + l * 64 + ((p ^ (l >> 1)) & 3) * 16) = pack16<T>(v + c0 + p * EACH);
+        __syncwarp();
+        if (vec && cols >= c0 + W) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const int r = p * 8 + (l >> 2);
+                uint4 u = *reinterpret_cast<const uint4*>(me.xpose + r * 64 + (((l & 3) ^ (r >> 1)) & 3) * 16);
+                if (r >= rows) continue;
+                uint4* to = reinterpret_cast<uint4*>(out + (int64_t)r * ld + c0 + (l & 3) * EACH);
+                if (ADD) {
+                    const uint4 o = *to;
+                    u.x = __float_as_uint(__uint_as_float(u.x) + __uint_as_float(o.x));
+                    u.y = __float_as_uint(__uint_as_float(u.y) + __uint_as_float(o.y));
+                    u.z = __float_as_uint(__uint_as_float(u.z) + __uint_as_float(o.z));
+                    u.w = __float_as_uint(__uint_as_float(u.w) + __uint_as_float(o.w));
+                }
+                *to = u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int r = i * (32 / W) + l / W, c = l % W;
+                if (r < rows && c0 + c < cols)
+                    out[(int64_t)r * ld + c0 + c] = reinterpret_cast<const T*>(
+                        me.xpose + r * 64 + (((c / EACH) ^ (r >> 1)) & 3) * 16)[c % EACH];
+            }
+        }
+    }
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: start address, leading and
@@ -258,8 +320,8 @@ struct Ctx {
 //   a_mn(t), b_mn(t)       operand majors of a tile
 //   bytes(t)               bytes this CTA loads per block
 //   load(t, kb, sa, sb, bar, ctx)
-//   zero(t, row, half, ctx)                                    the epilogue of a tile without blocks
-//   epilogue(t, tmem, row, half, ctx)                          !PROMOTE
+//   zero(t, me, ctx)                                    the epilogue of a tile without blocks
+//   epilogue(t, tmem, me, ctx)                          !PROMOTE
 //   group(), Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulator is
 //                          read back and joined in registers after each `group` blocks
 template <typename Op>
@@ -268,7 +330,8 @@ __device__ __forceinline__ void run(const Op& op) {
     using G = Geo<CG>;
     extern __shared__ uint8_t raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    Ring* ring = reinterpret_cast<Ring*>(base + (size_t)G::STAGES * G::STAGE);
+    uint8_t* xpose = base + (size_t)G::STAGES * G::STAGE;
+    Ring* ring = reinterpret_cast<Ring*>(xpose + EPI_WARPS * XPOSE);
     const uint32_t stages = smem_u32(base);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Ctx ctx;
@@ -301,7 +364,7 @@ __device__ __forceinline__ void run(const Op& op) {
 
     Tile t;
     if (warp < EPI_WARP0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // Both roles run as whole warps with one elected thread at the loads and MMAs:
         // addresses and descriptors then stay in uniform registers, which those
         // instructions want (from a single-thread branch a block's four MMAs took
@@ -377,40 +440,45 @@ __device__ __forceinline__ void run(const Op& op) {
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        const int quad = warp & 3, half = (warp - EPI_WARP0) >> 2;
-        const int row = (int)ctx.rank * 128 + quad * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        Lane me;
+        me.lane = lane;
+        me.quad = warp & 3;
+        me.grp = (warp - EPI_WARP0) >> 2;
+        me.row = (int)ctx.rank * 128 + me.quad * 32 + lane;
+        me.xpose = xpose + (warp - EPI_WARP0) * XPOSE;
+        const uint32_t lanes = (uint32_t)(me.quad * 32) << 16;
         const uint32_t te0 = CG == 2 ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
         uint32_t buf = 0, tph = 0;
         bool ok = true;
         for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
+            t.seq = i;
             if (t.kn == 0) {  // an empty sum: no product, no accumulator
-                op.zero(t, row, half, ctx);
+                op.zero(t, me, ctx);
                 continue;
             }
             if constexpr (Op::PROMOTE) {
                 typename Op::Acc acc;
-                op.begin(acc, t, row, half, ctx);
+                op.begin(acc, t, me, ctx);
                 for (int kb = 0; kb < t.kn; kb += op.group()) {
-                    op.prepare(acc, t, t.k0 + kb, row, half, ctx);
+                    op.prepare(acc, t, t.k0 + kb, me, ctx);
                     ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                     if (!ok) break;
                     fence_after();
                     // the accumulator goes back to the MMAs as soon as it has been read
-                    op.join(acc, t, tmem + buf * 256 + lanes, row, half, ctx, [&] {
+                    op.join(acc, t, tmem + buf * 256 + lanes, me, ctx, [&] {
                         fence_before();
                         __syncwarp();
                         if (lane == 0) arrive_remote(te0 + buf * 8);
                     });
                     if (++buf == 2) buf = 0, tph ^= 1;
                 }
-                if (ok) op.finish(acc, t, row, half, ctx);
+                if (ok) op.finish(acc, t, me, ctx);
             } else {
                 ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                 if (!ok) break;
                 fence_after();
-                op.epilogue(t, tmem + buf * 256 + lanes, row, half, ctx);
+                op.epilogue(t, tmem + buf * 256 + lanes, me, ctx);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_remote(te0 + buf * 8);

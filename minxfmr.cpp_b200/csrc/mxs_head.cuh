@@ -25,11 +25,11 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 
-// Eight values rounded to two-byte ones.
+// Sixteen bytes of values, rounded to their type.
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* v);
+__device__ __forceinline__ uint4 pack16(const float* v);
 template <>
-__device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float* v) {
+__device__ __forceinline__ uint4 pack16<__nv_bfloat16>(const float* v) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -39,7 +39,7 @@ __device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float* v) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <>
-__device__ __forceinline__ uint4 pack8<__half>(const float* v) {
+__device__ __forceinline__ uint4 pack16<__half>(const float* v) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -48,30 +48,9 @@ __device__ __forceinline__ uint4 pack8<__half>(const float* v) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-// 32 values to `out`, `n` of them inside the row, as 16-byte stores where `vec` says that they are aligned.
-template <typename T>
-__device__ __forceinline__ void store32(T* out, const float (&v)[32], int n, bool vec) {
-    if (vec && n >= 32) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) *reinterpret_cast<uint4*>(out + j) = pack8<T>(v + j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < n) out[j] = from_f32<T>(v[j]);
-    }
-}
 template <>
-__device__ __forceinline__ void store32<float>(float* out, const float (&v)[32], int n, bool vec) {
-    if (vec && n >= 32) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(out + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < n) out[j] = v[j];
-    }
+__device__ __forceinline__ uint4 pack16<float>(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
 }
 
 inline int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
