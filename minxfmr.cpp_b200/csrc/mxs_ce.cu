@@ -188,6 +188,7 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, 2^-22 relative; results
 template <int CG_>
 struct LogitTiles {
     static constexpr int CG = CG_;
+    static constexpr int EPI = 16;
     static constexpr bool F8 = false, PROMOTE = false;
     __device__ int group() const { return INT32_MAX; }
     CUtensorMap mh, mw;
@@ -253,13 +254,10 @@ struct ScoreOp : LogitTiles<CG_> {
             for (int i = 0; i < 2; ++i) {
                 const int c0 = me.grp * 32 + i * 128;
                 if (c0 < t.n) {
+                    float v[32];
+                    mxs::gemm::tmem_ld32(tmem + c0, v);
 #pragma unroll
-                    for (int h = 0; h < 32; h += 16) {
-                        float v[16];
-                        mxs::gemm::tmem_ld16(tmem + c0 + h, v);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) a.v[i][h + j] += v[j];
-                    }
+                    for (int j = 0; j < 32; ++j) a.v[i][j] += v[j];
                 }
             }
         }
@@ -402,6 +400,7 @@ struct GradLogitsOp : LogitTiles<CG_> {
 template <typename T>
 struct ProductOp {
     static constexpr int CG = 2;
+    static constexpr int EPI = 16;
     static constexpr bool F8 = false, PROMOTE = false;
     __device__ int group() const { return INT32_MAX; }
     CUtensorMap g_k, g_m, w_n, h_n;

@@ -220,14 +220,20 @@ cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
 // 256 of accumulator reads and 256 of FMA a scheduler).
 // ---------------------------------------------------------------------------
 
-template <int CG_, typename O>
+// RUNS: runs of 32 columns a thread holds, 4 for tiles of up to 256 columns, 2 for
+// up to 128. The join has no branch around the sums (a warp without rows joins what
+// it finds and stores nothing): where two paths meet the compiler copies all 128.
+template <int CG_, typename O, int RUNS>
 struct MatmulOp {
     static constexpr int CG = CG_;
+    static constexpr int EPI = 8;
     static constexpr bool F8 = true, PROMOTE = true;
     __device__ int group() const { return 1; }
     struct Acc {
-        float v[2][32];
-        float row_next, next[2], now[2];  // scales of the next block and of this one
+        float v[RUNS][32];
+        const float *ra, *rb[RUNS];          // scales of this row, and of the runs of columns
+        float row_next, next[RUNS];       // those of the next block
+        float now[RUNS];                  // their products for this one
     };
     CUtensorMap ma, mb;
     int format;
@@ -259,70 +265,70 @@ struct MatmulOp {
         mxs::gemm::tma_load<CG>(s_b, &mb, k * BLK, t.n0 + (int)x.rank * (n / CG), bar);
     }
     __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
-    __device__ void fetch(Acc& a, const Tile& t, int k, const Lane& me) const {
-        a.row_next = sa[(int64_t)min(rows - 1, t.m0 + me.row) * kb + k];
+    __device__ void fetch(Acc& a, int k) const {
+        a.row_next = a.ra[k];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c0 = min(cols - 1, t.n0 + me.grp * 32 + i * 128);  // 32 columns lie in one block of 128
-            a.next[i] = sb[(int64_t)(c0 / BLK) * kb + k];
-        }
+        for (int i = 0; i < RUNS; ++i) a.next[i] = a.rb[i][k];
     }
     __device__ void begin(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) a.v[i / 32][i % 32] = 0.0f;
-        fetch(a, t, 0, me);
-    }
-    __device__ void prepare(Acc& a, const Tile& t, int k, const Lane& me, const Ctx&) const {
+        for (int i = 0; i < 32 * RUNS; ++i) a.v[i / 32][i % 32] = 0.0f;
+        a.ra = sa + (int64_t)min(rows - 1, t.m0 + me.row) * kb;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) a.now[i] = a.row_next * a.next[i];
-        if (k + 1 < kb) fetch(a, t, k + 1, me);
+        for (int i = 0; i < RUNS; ++i)  // 32 columns lie in one block of 128
+            a.rb[i] = sb + (int64_t)(min(cols - 1, t.n0 + me.grp * 32 + i * 64) / BLK) * kb;
+        fetch(a, 0);
+    }
+    __device__ void prepare(Acc& a, const Tile&, int k, const Lane&, const Ctx&) const {
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) a.now[i] = a.row_next * a.next[i];
+        fetch(a, min(k + 1, kb - 1));
     }
     template <typename Release>
     __device__ void join(Acc& a, const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, Release release) const {
-        const int c0 = me.grp * 32;
-        if (((t.m0 + me.row) & ~31) >= rows || c0 >= t.n) {  // no row or column of this warp
-            release();
-            return;
+        // the next run is on its way while one is joined; a run past the tile's is not kept
+        const int c0 = me.grp * 32, end = t.n - 32;
+        float x[32], y[32];
+        auto add = [&](int i, const float (&p)[32]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(p[j], a.now[i], a.v[i][j]);
+        };
+        mxs::gemm::tmem_ld32(tmem + min(c0, end), x);
+        mxs::gemm::tmem_ld32(tmem + min(c0 + 64, end), y);
+        if (RUNS == 4) {
+            add(0, x);
+            mxs::gemm::tmem_ld32(tmem + min(c0 + 128, end), x);
+            add(1, y);
+            mxs::gemm::tmem_ld32(tmem + min(c0 + 192, end), y);
         }
-        const int runs = c0 + 128 < t.n ? 2 : 1;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (i >= runs) break;
-#pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-                float v[16];
-                mxs::gemm::tmem_ld16(tmem + c0 + i * 128 + h, v);
-                if (h == 16 && i == runs - 1) release();
-#pragma unroll
-                for (int j = 0; j < 16; j += 2)
-                    mxs::gemm::fma2(a.v[i][h + j], a.v[i][h + j + 1], v[j], v[j + 1], a.now[i]);
-            }
-        }
+        release();
+        add(RUNS - 2, x);
+        add(RUNS - 1, y);
     }
     __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
         const int r0 = t.m0 + me.row - me.lane;
         if (r0 >= rows) return;
         O* o = out + (int64_t)r0 * ldo + t.n0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c0 = me.grp * 32 + i * 128;
-            if (c0 < t.n)
-                mxs::gemm::store_rows<O, false>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
+        for (int i = 0; i < RUNS; ++i) {
+            const int c0 = me.grp * 32 + i * 64;
+            if (c0 >= t.n) break;
+            mxs::gemm::store_rows<O, false>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
         }
     }
 };
 
-template <int CG, typename O>
-int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
-                  int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
-    MatmulOp<CG, O> op{};
+template <int CG, typename O, int RUNS>
+int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
+                 int64_t n, int64_t k, void* out, int64_t ldo, int width, int sms, uint32_t* status, cudaStream_t st) {
+    MatmulOp<CG, O, RUNS> op{};
     op.format = 0;
     op.drop = mxs::test_drop_tile();
     op.status = status;
     op.sa = sa, op.sb = sb;
     op.rows = (int)rows, op.cols = (int)n, op.kb = (int)ceil_div(k, BLK);
     op.mt = (int)ceil_div(rows, 128 * CG);
-    op.n = mxs::tile_width(op.mt, n, sms / CG, 64, 32);
+    op.n = width;
     op.nt = (int)ceil_div(n, op.n);
     op.a_rows = CG == 1 ? (int)round_up(rows, 8) : 128;
     op.out = static_cast<O*>(out);
@@ -333,6 +339,16 @@ int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, in
         return MXS_ERR_CUDA;
     const int64_t tiles = (int64_t)op.mt * op.nt;
     return mxs::gemm::launch(op, (int)std::min<int64_t>(sms / CG, tiles), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+}
+
+template <typename O>
+int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
+                  int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
+    const int cg = rows > 128 ? 2 : 1;
+    const int w = mxs::tile_width(ceil_div(rows, 128 * cg), n, sms / cg, 64, 32);
+    auto go = [&](auto f) { return f(a, lda, sa, b, ldb, sb, rows, n, k, out, ldo, w, sms, status, st); };
+    if (cg == 2) return w > 128 ? go(launch_tiles<2, O, 4>) : go(launch_tiles<2, O, 2>);
+    return w > 128 ? go(launch_tiles<1, O, 4>) : go(launch_tiles<1, O, 2>);
 }
 
 bool bad_type(int t) { return t != MXS_BF16 && t != MXS_F16 && t != MXS_F32; }
@@ -439,15 +455,12 @@ int mxs_matmul_fp8(const void* d_a, int64_t ld_a, const float* d_a_scale, const 
         if (mxs::copy_rows(d_b, ld_b, cp.b, ldk, n, k, sms, st) != cudaSuccess) return MXS_ERR_CUDA;
         d_b = cp.b, ld_b = ldk;
     }
-    const bool pair = rows > 128;
-    auto go = [&](auto tag) {
-        using O = decltype(tag);
-        return pair ? launch_matmul<2, O>(d_a, ld_a, d_a_scale, d_b, ld_b, d_b_scale, rows, n, k, d_out, ld_out, sms,
-                                          status, st)
-                    : launch_matmul<1, O>(d_a, ld_a, d_a_scale, d_b, ld_b, d_b_scale, rows, n, k, d_out, ld_out, sms,
-                                          status, st);
+    auto go = [&](auto f) {
+        return f(d_a, ld_a, d_a_scale, d_b, ld_b, d_b_scale, rows, n, k, d_out, ld_out, sms, status, st);
     };
-    return out_dtype == MXS_F32 ? go(0.0f) : out_dtype == MXS_BF16 ? go(__nv_bfloat16()) : go(__half());
+    return out_dtype == MXS_F32    ? go(launch_matmul<float>)
+           : out_dtype == MXS_BF16 ? go(launch_matmul<__nv_bfloat16>)
+                                   : go(launch_matmul<__half>);
 }
 
 int mxs_sample_from_hidden_fp8_workspace_size(const void* d_weight_q, int64_t ld_weight, int64_t rows, int64_t d_model,

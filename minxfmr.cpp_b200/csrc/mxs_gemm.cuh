@@ -3,21 +3,22 @@
 //
 //   warp 0      loads operand tiles (TMA, 128-byte swizzle) into a ring of stages
 //   warp 1      issues tcgen05.mma (one thread), accumulators in TMEM
-//   warps 4..19 read accumulators back (tcgen05.ld) and do the Op's epilogue: four
-//               warps share the 32 rows that the hardware gives a warp's place, in
-//               four column groups of 32 (a thread has up to two runs of 32 columns)
+//   warps 4..   (Op::EPI of them, 8 or 16) read accumulators back (tcgen05.ld) and do
+//               the Op's epilogue: EPI / 4 warps share the 32 rows that the hardware
+//               gives a warp's place, each taking every (EPI / 4)-th run of 32 columns
 //
-// Sixteen epilogue warps, not eight, because a read of an accumulator takes some
-// hundred clocks and only other warps can fill them. Warps 0..3 give up registers
-// for them (setmaxnreg): 640 threads x 96 at launch = 128 x 64 + 512 x 104.
+// Warps 0..3 give up registers for the epilogue's (setmaxnreg). With 16 epilogue
+// warps: 640 threads x 96 at launch = 128 x 64 + 512 x 104; with 8: 384 x 168 =
+// 128 x 56 + 256 x 224. Sixteen suit epilogues with many instructions, eight the
+// 8-bit product, which keeps 128 sums a thread and loads in flight beside them.
 //
 // A tile is 128 rows per CTA by up to 256 columns. With CG = 2 a pair of CTAs
 // works on one 256-row tile: each loads its 128 rows of A and half of B's
 // columns, the even CTA issues the pair's MMAs, and every operand byte crosses
 // L2 -> shared memory once for 256 x 256 outputs (64 bytes per clock and SM at
 // full MMA rate, against 96 for a single CTA's 128 x 256, which L2 does not
-// deliver). TMEM's 512 columns hold two accumulators, so the epilogue of one
-// tile runs under the products of the next.
+// deliver). TMEM's 512 columns hold two accumulators of 256 columns, four of 128
+// or eight of 64, so the epilogue of one runs under the products of the next.
 //
 // Operands are held with 128 bytes of the contiguous direction per row, either
 // along K ("K-major": 64 16-bit or 128 8-bit values of K in a row) or along the
@@ -40,19 +41,19 @@
 namespace mxs {
 namespace gemm {
 
-constexpr int THREADS = 640;
 constexpr int EPI_WARP0 = 4;
-constexpr int EPI_WARPS = 16;
+constexpr int MAX_ACC = 8;  // accumulators that TMEM holds at most
 constexpr int XPOSE = 2048;  // bytes of shared memory for each epilogue warp's transposes
 constexpr int A_BYTES = 128 * 128;
 constexpr int ROW = 128;  // bytes of a stage row (one swizzle row)
 
-template <int CG>
+template <typename Op>
 struct Geo {
+    static constexpr int CG = Op::CG, THREADS = 32 * (EPI_WARP0 + Op::EPI);
     static constexpr int B_BYTES = 256 / CG * ROW;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = 196608 / STAGE;  // 192 KB: 4 or 6
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + EPI_WARPS * XPOSE + 512;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + Op::EPI * XPOSE + 512;
 };
 
 struct Tile {
@@ -71,7 +72,7 @@ struct Lane {
 };
 
 struct Ring {
-    uint64_t full[6], empty[6], tfull[2], tempty[2], drain;
+    uint64_t full[6], empty[6], tfull[MAX_ACC], tempty[MAX_ACC], drain;
     uint32_t tmem;
     int dead;
 };
@@ -188,18 +189,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
-    uint32_t r[16];
+// The same as pairs of floats in 64-bit registers, for the paired multiply-add:
+// made inside the block, the pairs are the loaded registers themselves, without
+// moves. (The wait costs nothing here: the values' first use waits.)
+__device__ __forceinline__ void tmem_ld32_pairs(uint32_t addr, uint64_t (&p)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15},"
-        " [%16];\n"
-        " tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "{\n .reg .b32 t<32>;\n"
+        " tcgen05.ld.sync.aligned.32x32b.x32.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15,"
+        " t16, t17, t18, t19, t20, t21, t22, t23, t24, t25, t26, t27, t28, t29, t30, t31}, [%16];\n"
+        " tcgen05.wait::ld.sync.aligned;\n"
+        " mov.b64 %0, {t0, t1}; mov.b64 %1, {t2, t3}; mov.b64 %2, {t4, t5}; mov.b64 %3, {t6, t7};\n"
+        " mov.b64 %4, {t8, t9}; mov.b64 %5, {t10, t11}; mov.b64 %6, {t12, t13}; mov.b64 %7, {t14, t15};\n"
+        " mov.b64 %8, {t16, t17}; mov.b64 %9, {t18, t19}; mov.b64 %10, {t20, t21}; mov.b64 %11, {t22, t23};\n"
+        " mov.b64 %12, {t24, t25}; mov.b64 %13, {t26, t27}; mov.b64 %14, {t28, t29}; mov.b64 %15, {t30, t31};\n"
+        "}"
+        : "=l"(p[0]), "=l"(p[1]), "=l"(p[2]), "=l"(p[3]), "=l"(p[4]), "=l"(p[5]), "=l"(p[6]), "=l"(p[7]),
+          "=l"(p[8]), "=l"(p[9]), "=l"(p[10]), "=l"(p[11]), "=l"(p[12]), "=l"(p[13]), "=l"(p[14]), "=l"(p[15])
         : "r"(addr)
         : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // Whether the unrolled j is the value h, kept as a comparison (the compiler would
@@ -210,10 +217,17 @@ __device__ __forceinline__ bool is_column(int h, int j) {
     return d == 0;
 }
 
-// a * b + c on two pairs of floats.
-__device__ __forceinline__ void fma2(float& x, float& y, float a0, float a1, float b) {
-    asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %4};\n mov.b64 r, {%0, %1};\n"
-        " fma.rn.f32x2 r, p, q, r;\n mov.b64 {%0, %1}, r;\n}" : "+f"(x), "+f"(y) : "f"(a0), "f"(a1), "f"(b));
+// Pairs of floats in 64-bit registers.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
+    return p;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) {  // c += a * b
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
 
 // A warp's 32 x 32 values (a row a thread) to row-major memory, through its
@@ -310,9 +324,11 @@ struct Ctx {
 };
 
 // The kernel body. Op (a __grid_constant__ parameter) has
-//   CG, F8, PROMOTE        compile-time: CTAs per tile, 8-bit operands, join accumulators per k block
+//   CG, F8, PROMOTE, EPI   compile-time: CTAs per tile, 8-bit operands, join accumulators in registers,
+//                          epilogue warps
 //   format                 operand format of the instruction descriptor
 //   drop                   test hook: CTA 0's producer stops before this block (-1: off)
+//   n                      columns of a tile at most
 //   status                 the device's status word
 //   prefetch()             tensor-map prefetch
 //   kept()                 the row count
@@ -327,11 +343,11 @@ struct Ctx {
 template <typename Op>
 __device__ __forceinline__ void run(const Op& op) {
     constexpr int CG = Op::CG;
-    using G = Geo<CG>;
+    using G = Geo<Op>;
     extern __shared__ uint8_t raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* xpose = base + (size_t)G::STAGES * G::STAGE;
-    Ring* ring = reinterpret_cast<Ring*>(xpose + EPI_WARPS * XPOSE);
+    Ring* ring = reinterpret_cast<Ring*>(xpose + Op::EPI * XPOSE);
     const uint32_t stages = smem_u32(base);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Ctx ctx;
@@ -343,9 +359,9 @@ __device__ __forceinline__ void run(const Op& op) {
             mbar_init(&ring->full[i], 1);
             mbar_init(&ring->empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < MAX_ACC; ++i) {
             mbar_init(&ring->tfull[i], 1);
-            mbar_init(&ring->tempty[i], EPI_WARPS * CG);
+            mbar_init(&ring->tempty[i], Op::EPI * CG);
         }
         mbar_init(&ring->drain, 1);
         ring->dead = 0;
@@ -363,8 +379,12 @@ __device__ __forceinline__ void run(const Op& op) {
     ctx.kept = op.kept();
 
     Tile t;
+    const uint32_t acc_cols = op.n <= 64 ? 64 : op.n <= 128 ? 128 : 256, accs = 512 / acc_cols;
     if (warp < EPI_WARP0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if constexpr (Op::EPI == 16)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // Both roles run as whole warps with one elected thread at the loads and MMAs:
         // addresses and descriptors then stay in uniform registers, which those
         // instructions want (from a single-thread branch a block's four MMAs took
@@ -417,7 +437,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     const bool last = in + 1 == group || kb == t.kn - 1;
                     if (elect()) {
                         const uint64_t da = da0 + (uint64_t)(s * (G::STAGE >> 4)), db = db0 + (uint64_t)(s * (G::STAGE >> 4));
-                        const uint32_t d = tmem + buf * 256;
+                        const uint32_t d = tmem + buf * acc_cols;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mma<CG, Op::F8>(d, da + k * step_a, db + k * step_b, idesc, k > 0 || in > 0);
@@ -429,7 +449,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     if (++s == G::STAGES) s = 0, ph ^= 1;
                     if (last) {
                         in = 0;
-                        if (++buf == 2) buf = 0, tph ^= 1;
+                        if (++buf == accs) buf = 0, tph ^= 1;
                     }
                 }
             }
@@ -440,7 +460,10 @@ __device__ __forceinline__ void run(const Op& op) {
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        if constexpr (Op::EPI == 16)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         Lane me;
         me.lane = lane;
         me.quad = warp & 3;
@@ -466,23 +489,23 @@ __device__ __forceinline__ void run(const Op& op) {
                     if (!ok) break;
                     fence_after();
                     // the accumulator goes back to the MMAs as soon as it has been read
-                    op.join(acc, t, tmem + buf * 256 + lanes, me, ctx, [&] {
+                    op.join(acc, t, tmem + buf * acc_cols + lanes, me, ctx, [&] {
                         fence_before();
                         __syncwarp();
                         if (lane == 0) arrive_remote(te0 + buf * 8);
                     });
-                    if (++buf == 2) buf = 0, tph ^= 1;
+                    if (++buf == accs) buf = 0, tph ^= 1;
                 }
                 if (ok) op.finish(acc, t, me, ctx);
             } else {
                 ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                 if (!ok) break;
                 fence_after();
-                op.epilogue(t, tmem + buf * 256 + lanes, me, ctx);
+                op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_remote(te0 + buf * 8);
-                if (++buf == 2) buf = 0, tph ^= 1;
+                if (++buf == accs) buf = 0, tph ^= 1;
             }
         }
     }
@@ -503,7 +526,7 @@ __device__ __forceinline__ void run(const Op& op) {
 bool make_map(CUtensorMap* map, const void* base, int elem_bytes, int64_t cols, int64_t rows, int64_t ld, int box_rows);
 
 template <typename Op>
-__global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Op op) {
+__global__ void __launch_bounds__(Geo<Op>::THREADS, 1) kernel(const __grid_constant__ Op op) {
     run(op);
 }
 
@@ -517,14 +540,14 @@ cudaError_t launch(const Op& op, int units, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!(configured.load(std::memory_order_relaxed) >> dev & 1)) {
-        e = cudaFuncSetAttribute(kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<CG>::SMEM);
+        e = cudaFuncSetAttribute(kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<Op>::SMEM);
         if (e != cudaSuccess) return e;
         configured.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(units * CG);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Geo<CG>::SMEM;
+    cfg.blockDim = dim3(Geo<Op>::THREADS);
+    cfg.dynamicSmemBytes = Geo<Op>::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
