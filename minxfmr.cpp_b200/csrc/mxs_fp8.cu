@@ -55,6 +55,34 @@ __device__ __forceinline__ void values(const Raw<float>& x, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
 }
+// The largest magnitude as the type's own bits without the sign, which order as
+// the magnitudes do, infinities and then NaN above every number; two 16-bit
+// types in a word, each half by itself.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Raw<T>& x) {
+    const uint4& u = x.u[0];
+    constexpr uint32_t M = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(u.x & M, u.y & M), __vmaxu2(u.z & M, u.w & M));
+}
+template <>
+__device__ __forceinline__ uint32_t top_bits<float>(const Raw<float>& x) {
+    constexpr uint32_t M = 0x7fffffffu;
+    const uint4 &u = x.u[0], &w = x.u[1];
+    return max(max(max(u.x & M, u.y & M), max(u.z & M, u.w & M)), max(max(w.x & M, w.y & M), max(w.z & M, w.w & M)));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t max_bits<float>(uint32_t a, uint32_t b) { return max(a, b); }
+// Of the (halves of the) word: the magnitude, and whether it is no number.
+__device__ __forceinline__ float magnitude(uint32_t m, const __nv_bfloat16*) {
+    return __uint_as_float(max(m << 16, m & 0xffff0000u));
+}
+__device__ __forceinline__ float magnitude(uint32_t m, const __half*) {
+    return __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+}
+__device__ __forceinline__ float magnitude(uint32_t m, const float*) { return __uint_as_float(m); }
+
 // 16-byte loads where the eight are aligned and inside the row; zeros outside.
 template <typename T>
 __device__ __forceinline__ Raw<T> load8(const T* x, int n, bool vec) {
@@ -85,24 +113,19 @@ __device__ __forceinline__ uint32_t quad(const float* y) {
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
-// The other blocks (a scale below 2^-90, or an infinity): one division each.
-template <typename T>
-__device__ __noinline__ uint2 divide8(const Raw<T> x, float s) {
-    float v[8];
-    values(x, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] / s;
-    return make_uint2(quad(v), quad(v + 4));
-}
 
-// Bound by memory: each value is read once and kept in registers between its
-// block's maximum and its rounding. ROWS_OF = 1: sixteen lanes hold a block of
-// 128, a warp two neighbouring ones, twice. ROWS_OF = 128: a CTA of 256 threads
-// holds a block, sixteen lanes a row, eight rows each.
+// Bound by memory: each value is read once and kept in registers, in its own type,
+// between its block's maximum and its rounding. ROWS_OF = 1: sixteen lanes hold a
+// block of 128, a warp two neighbouring ones, twice. ROWS_OF = 128: a CTA of 256
+// threads holds a block, sixteen lanes a row, eight rows each. A block with an
+// infinity or NaN, or with a scale below 2^-90, is read again and divided value
+// by value.
 template <typename T, int ROWS_OF>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, int rows, int cols, uint8_t* q,
-                                                       int64_t ldq, float* scale, bool vec_in, bool vec_out) {
-    constexpr int HELD = ROWS_OF == 1 ? 2 : 8;
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
+    quantize_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
+                    float* __restrict__ scale, bool vec_in, bool vec_out) {
+    constexpr int HELD = ROWS_OF == 1 ? 2 : 8, TOPS = ROWS_OF == 1 ? HELD : 1;
+    constexpr int DR = ROWS_OF == 1 ? 0 : 16, DC = ROWS_OF == 1 ? 2 * BLK : 0;
     const int tid = threadIdx.x, lane = tid & 31, sub = tid & 15;
     const int bc = (cols + BLK - 1) / BLK;
     int row0, col0;  // of the first eight; the others follow 256 columns or 16 rows on
@@ -114,78 +137,93 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, 
         row0 = (blockIdx.x / bc) * BLK + (tid >> 4);
         col0 = (blockIdx.x % bc) * BLK + sub * 8;
     }
-    constexpr int DR = ROWS_OF == 1 ? 0 : 16, DC = ROWS_OF == 1 ? 2 * BLK : 0;
     auto inside = [&](int i) { return row0 + i * DR < rows ? min(8, cols - col0 - i * DC) : 0; };  // may be negative
+    const T* from = x + (int64_t)row0 * ldx + col0;
+    uint8_t* to = q + (int64_t)row0 * ldq + col0;
+    auto put = [&](int i, int n, uint2 w) {
+        uint8_t* p = to + (int64_t)(i * DR) * ldq + i * DC;
+        if (vec_out && n >= 8) {
+            *reinterpret_cast<uint2*>(p) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) p[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+        }
+    };
     Raw<T> v[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int n = inside(i);
-        v[i] = load8(n > 0 ? x + (int64_t)(row0 + i * DR) * ldx + col0 + i * DC : x, n, vec_in);
+        v[i] = load8(n > 0 ? from + (int64_t)(i * DR) * ldx + i * DC : x, n, vec_in);
     }
-    constexpr int TOPS = ROWS_OF == 1 ? HELD : 1;
-    __shared__ float s_top[2][8];
-    float top[TOPS];
-    bool inf = false;
-    for (int pass = 0; pass < 2; ++pass) {  // the second pass leaves infinities out, where there are any
-        bool more = false;
-#pragma unroll
-        for (int i = 0; i < TOPS; ++i) top[i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            float f[8];
-            values(v[i], f);
-            float m = top[i % TOPS];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {  // a NaN is not a maximum
-                const float a = fabsf(f[j]);
-                m = fmaxf(m, pass == 0 || a <= FLT_MAX ? a : 0.0f);
-            }
-            top[i % TOPS] = m;
-        }
-#pragma unroll
-        for (int i = 0; i < TOPS; ++i) {
-#pragma unroll
-            for (int o = 8; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-            if (ROWS_OF != 1) {
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-                if (lane == 0) s_top[pass][tid >> 5] = top[i];
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < 8; ++w) top[i] = fmaxf(top[i], s_top[pass][w]);
-            }
-            more |= top[i] > FLT_MAX;
-        }
-        if (!__any_sync(0xffffffffu, more)) break;  // ROWS_OF 128: the whole CTA agrees
-        inf = true;
-    }
+    __shared__ uint32_t s_top[8];
+    __shared__ float s_slow[8];
+    uint32_t bits[TOPS];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const int n = inside(i);
-        if (n <= 0) continue;
-        const int row = row0 + i * DR, col = col0 + i * DC;
-        const float s = block_scale(top[i % TOPS]);
-        const float r = 1.0f / s;
-        uint2 w;
-        if (inf || s < 8.0779357e-28f) {  // 2^-90
-            w = divide8(v[i], s);
-        } else {
-            float y[8];
-            values(v[i], y);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = quotient(y[j], s, r);
-            w = make_uint2(quad(y), quad(y + 4));
-        }
-        uint8_t* to = q + (int64_t)row * ldq + col;
-        if (vec_out && n >= 8) {
-            *reinterpret_cast<uint2*>(to) = w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < n) to[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
-        }
-        if (ROWS_OF == 1 && sub == 0) scale[(int64_t)row * bc + col / BLK] = s;
+        const uint32_t t = top_bits(v[i]);
+        bits[i % TOPS] = i < TOPS ? t : max_bits<T>(bits[i % TOPS], t);
     }
-    if (ROWS_OF != 1 && tid == 0) scale[blockIdx.x] = block_scale(top[0]);
+#pragma unroll
+    for (int i = 0; i < TOPS; ++i) {
+#pragma unroll
+        for (int o = 8; o; o >>= 1) bits[i] = max_bits<T>(bits[i], __shfl_xor_sync(0xffffffffu, bits[i], o));
+        if (ROWS_OF != 1) {
+            bits[i] = max_bits<T>(bits[i], __shfl_xor_sync(0xffffffffu, bits[i], 16));
+            if (lane == 0) s_top[tid >> 5] = bits[i];
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 8; ++w) bits[i] = max_bits<T>(bits[i], s_top[w]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TOPS; ++i) {
+        const float top = magnitude(bits[i], static_cast<const T*>(nullptr));
+        float s = block_scale(top);
+        // ROWS_OF 1: one of the warp's blocks, so that the warp stays together; 128: the whole CTA agrees
+        if (__any_sync(0xffffffffu, !(top <= FLT_MAX) || s < 8.0779357e-28f)) {  // 2^-90
+            float m = 0.0f;
+            for (int h = i; h < HELD; h += TOPS) {
+                const int n = inside(h);
+                for (int j = 0; j < n; ++j) {
+                    const float a = fabsf(to_f32(from[(int64_t)(h * DR) * ldx + h * DC + j]));
+                    if (a <= FLT_MAX) m = fmaxf(m, a);
+                }
+            }
+#pragma unroll
+            for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (ROWS_OF != 1) {
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                if (lane == 0) s_slow[tid >> 5] = m;
+                __syncthreads();
+                for (int w = 0; w < 8; ++w) m = fmaxf(m, s_slow[w]);
+            }
+            s = block_scale(m);
+            for (int h = i; h < HELD; h += TOPS) {
+                const int n = inside(h);
+                if (n <= 0) continue;
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    y[j] = j < n ? to_f32(from[(int64_t)(h * DR) * ldx + h * DC + j]) / s : 0.0f;
+                put(h, n, make_uint2(quad(y), quad(y + 4)));
+            }
+        } else {
+            const float r = 1.0f / s;
+#pragma unroll
+            for (int h = i; h < HELD; h += TOPS) {
+                const int n = inside(h);
+                if (n <= 0) continue;
+                float y[8];
+                values(v[h], y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = quotient(y[j], s, r);
+                put(h, n, make_uint2(quad(y), quad(y + 4)));
+            }
+        }
+        if (ROWS_OF != 1 ? tid == 0 : sub == 0 && inside(i) > 0)
+            scale[ROWS_OF != 1 ? (int64_t)blockIdx.x : (int64_t)row0 * bc + (col0 + i * DC) / BLK] = s;
+    }
 }
 
 template <typename T>
