@@ -81,62 +81,65 @@ __device__ __forceinline__ bool kept_row(const Pack& p, int64_t r) {
 }
 
 constexpr int PACK_T = 256;
-constexpr int PACK_TAIL = 256;  // rows after the last kept one that read zero
+constexpr int PACK_ROWS = 256;  // packed rows are allocated in multiples of this
 
 // Each CTA packs a contiguous range of rows; it counts the kept rows before its
-// range itself (a few KB of targets from L2), so one launch does it all.
+// range itself (a few KB of targets from L2), so one launch does it all. In
+// backward every CTA scans all rows (for the largest gradient weight) and so
+// knows how many are kept: together they zero the rows up to the next multiple
+// of 64, which grad_weight's product reads as its last block of K.
 template <typename T>
 __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
+    mxs::gemm::grid_wait();
     mxs::gemm::grid_launch_dependents();
-    __shared__ int s_cnt[PACK_T / 32];
+    __shared__ int s_cnt[PACK_T / 32], s_all[PACK_T / 32], s_pos[PACK_T];
     __shared__ float s_max[PACK_T / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (int)ceil_div(p.rows, gridDim.x);
     const int r0 = min(p.rows, (int)blockIdx.x * per), r1 = min(p.rows, r0 + per);
-    int n = 0;
+    int n = 0, all = 0;
     float gm = 0.0f;
     const int scan_to = p.grad ? p.rows : r0;
+#pragma unroll 4
     for (int r = tid; r < scan_to; r += PACK_T) {
-        if (!kept_row(p, r)) continue;
-        if (r < r0) ++n;
-        if (p.grad) {
-            const float g = fabsf(p.grad[r]);
-            if (g <= FLT_MAX) gm = fmaxf(gm, g);
-        }
+        const bool keep = kept_row(p, r);
+        const float g = p.grad ? fabsf(p.grad[r]) : 0.0f;
+        all += keep;
+        n += keep && r < r0;
+        if (keep && g <= FLT_MAX) gm = fmaxf(gm, g);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         n += __shfl_xor_sync(0xffffffffu, n, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
         gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
     }
-    if (lane == 0) {
-        s_cnt[warp] = n;
-        s_max[warp] = gm;
-    }
+    if (lane == 0) s_cnt[warp] = n, s_all[warp] = all, s_max[warp] = gm;
     __syncthreads();
-    n = 0;
+    n = all = 0;
     gm = 0.0f;
     for (int w = 0; w < PACK_T / 32; ++w) {
         n += s_cnt[w];
+        all += s_all[w];
         gm = fmaxf(gm, s_max[w]);
     }
     if (!(gm > 0.0f)) gm = 1.0f;
     int base = n;
-    const int step = 16 / sizeof(T);
-    const bool vec = reinterpret_cast<uintptr_t>(p.hidden) % 16 == 0 && p.ld_hidden % step == 0;
+    constexpr int STEP = 16 / sizeof(T);
+    const bool vec = reinterpret_cast<uintptr_t>(p.hidden) % 16 == 0 && p.ld_hidden % STEP == 0;
     for (int c0 = r0; c0 < r1; c0 += PACK_T) {
-        __syncthreads();
         const int r = c0 + tid;
         const bool keep = r < r1 && kept_row(p, r);
         const uint32_t b = __ballot_sync(0xffffffffu, keep);
+        __syncthreads();
         if (lane == 0) s_cnt[warp] = __popc(b);
         __syncthreads();
-        int at = base + __popc(b & ((1u << lane) - 1));
-        int all = 0;
+        int at = base + __popc(b & ((1u << lane) - 1)), here = 0;
         for (int w = 0; w < PACK_T / 32; ++w) {
             if (w < warp) at += s_cnt[w];
-            all += s_cnt[w];
+            here += s_cnt[w];
         }
+        s_pos[tid] = keep ? at : -1;
         if (r < r1) p.pos[r] = keep ? at : -1;
         if (keep) {
             p.target[at] = (int)target_of(p, r);
@@ -145,31 +148,33 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
                 p.ghat[at] = p.grad[r] / gm;
             }
         }
-        base += all;
-        // the rows themselves: a warp each, positions recomputed from the ballots' order
+        base += here;
         __syncthreads();
+        // the rows themselves, a warp each
         for (int i = warp; i < min(PACK_T, r1 - c0); i += PACK_T / 32) {
-            const int to = p.pos[c0 + i];
+            const int to = s_pos[i];
             if (to < 0) continue;
             const T* src = static_cast<const T*>(p.hidden) + (int64_t)(c0 + i) * p.ld_hidden;
             T* dst = static_cast<T*>(p.packed) + (int64_t)to * p.ldk;
-            int k = 0;
+            int k = lane;
             if (vec) {
-                for (k = lane * step; k + step <= p.d; k += 32 * step)
-                    *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
-                k = p.d / step * step;
+#pragma unroll 4
+                for (int j = lane; j < p.d / STEP; j += 32)
+                    reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(src)[j];
+                k += p.d / STEP * STEP;
             }
-            for (k += lane; k < p.d; k += 32) dst[k] = src[k];
+            for (; k < p.d; k += 32) dst[k] = src[k];
         }
     }
-    if (r1 == p.rows && r0 < r1) {  // the range that ends the rows knows how many were kept
-        if (tid == 0) {
-            p.head->kept = base;
-            p.head->gmax = gm;
-        }
-        const int end = (int)((base + (int64_t)PACK_TAIL - 1) / PACK_TAIL * PACK_TAIL);
-        for (int64_t i = tid; i < (int64_t)(end - base) * p.ldk; i += PACK_T)
-            static_cast<T*>(p.packed)[(int64_t)base * p.ldk + i] = mxs::from_f32<T>(0.0f);
+    if (p.grad) {
+        const int64_t words = (int64_t)((64 - all % 64) % 64) * p.ldk / STEP;  // ldk is a multiple of 8
+        uint4* tail = reinterpret_cast<uint4*>(static_cast<T*>(p.packed) + (int64_t)all * p.ldk);
+        for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; i < words; i += (int64_t)gridDim.x * PACK_T)
+            tail[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (r1 == p.rows && r0 < r1 && tid == 0) {  // the range that ends the rows knows how many were kept
+        p.head->kept = base;
+        p.head->gmax = gm;
     }
 }
 
@@ -314,34 +319,46 @@ struct ScoreOp : LogitTiles<CG_> {
     }
 };
 
-// One warp per row joins the tiles' pairs, in the same order every time.
+__device__ __forceinline__ void join_pair(float& m, float& s, float om, float os) {
+    const float nm = fmaxf(m, om), sub = nm == -INFINITY ? 0.0f : nm;
+    s = s * exp2f(m - sub) + os * exp2f(om - sub);
+    m = nm;
+}
+
+// Joins the tiles' pairs of a row, in the same order every time: a warp per row,
+// or (whole: few rows, where a warp's chain of reads would be most of the call)
+// a CTA.
 __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, const float* ytarget, const int* pos,
-                                                         int rows, int tiles, float* loss, float* lse) {
-    const int lane = threadIdx.x & 31;
-    const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+                                                         int rows, int tiles, bool whole, float* loss, float* lse) {
+    __shared__ float2 s_pair[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = whole ? blockIdx.x : blockIdx.x * 8 + warp;
     mxs::gemm::grid_wait();
+    mxs::gemm::grid_launch_dependents();
     if (r >= rows) return;
     const int at = pos[r];
     if (at < 0) {
-        if (lane == 0) {
+        if (whole ? threadIdx.x == 0 : lane == 0) {
             if (loss) loss[r] = 0.0f;
             if (lse) lse[r] = 0.0f;
         }
         return;
     }
     float m = -INFINITY, s = 0.0f;
-    for (int i = lane; i < tiles; i += 32) {
+    const int step = whole ? 256 : 32;
+#pragma unroll 4
+    for (int i = whole ? threadIdx.x : lane; i < tiles; i += step) {
         const float2 q = part[(int64_t)i * rows + at];
-        const float nm = fmaxf(m, q.x), sub = nm == -INFINITY ? 0.0f : nm;
-        s = s * exp2f(m - sub) + q.y * exp2f(q.x - sub);
-        m = nm;
+        join_pair(m, s, q.x, q.y);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-        const float nm = fmaxf(m, om), sub = nm == -INFINITY ? 0.0f : nm;
-        s = s * exp2f(m - sub) + os * exp2f(om - sub);
-        m = nm;
+    for (int o = 16; o; o >>= 1)
+        join_pair(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    if (whole) {
+        if (lane == 0) s_pair[warp] = make_float2(m, s);
+        __syncthreads();
+        if (threadIdx.x != 0) return;
+        for (int w = 1; w < 8; ++w) join_pair(m, s, s_pair[w].x, s_pair[w].y);
     }
     if (lane == 0) {
         const float y = ytarget[at];
@@ -512,22 +529,39 @@ struct ProductOp {
 // grad_hidden of every row: its tiles' splits added in order, times the scale
 // (rows left out: zero).
 template <typename T>
-__global__ void __launch_bounds__(256) grad_hidden_out_kernel(const float* acc, const int* pos, const Head* head,
+__global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, const int* pos, const Head* head,
                                                               int d, int n, int width, int units, float scale, T* out,
                                                               int64_t ld) {
     mxs::gemm::grid_wait();
-    const int64_t r = blockIdx.x;
+    mxs::gemm::grid_launch_dependents();
+    const int64_t r = blockIdx.y;
+    const int k = (blockIdx.x * 128 + threadIdx.x) * 4;  // four columns of one tile
+    if (k >= d) return;
     const int at = pos[r];
-    const float s = head->gmax * scale;
-    const int nt = (d + n - 1) / n, splits = grad_hidden_splits((head->kept + 255) / 256 * nt, width, units);
-    for (int k = threadIdx.x; k < d; k += 256) {
-        float v = 0.0f;
-        if (at >= 0) {
-            const int64_t tile = (int64_t)(at / 256) * nt + k / n;
-            const float* a = acc + (tile * splits * 256 + at % 256) * 256 + k % n;
-            for (int i = 0; i < splits; ++i) v += a[(int64_t)i * 65536];
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (at >= 0) {
+        const int nt = (d + n - 1) / n, splits = grad_hidden_splits((head->kept + 255) / 256 * nt, width, units);
+        const int64_t tile = (int64_t)(at / 256) * nt + k / n;
+        const float* a = acc + (tile * splits * 256 + at % 256) * 256 + k % n;
+#pragma unroll 8
+        for (int i = 0; i < splits; ++i) {
+            const float4 q = *reinterpret_cast<const float4*>(a + (int64_t)i * 65536);
+            v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
         }
-        out[r * ld + k] = mxs::from_f32<T>(at < 0 ? 0.0f : v * s);
+        const float s = head->gmax * scale;
+        v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
+    }
+    T* o = out + r * ld + k;
+    const float w[4] = {v.x, v.y, v.z, v.w};
+    if (k + 4 <= d && ld % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0) {
+        T t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = mxs::from_f32<T>(w[i]);
+        *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k + i < d) o[i] = mxs::from_f32<T>(w[i]);
     }
 }
 
@@ -558,7 +592,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     Plan pl{};
     Carve c(ws);
     rows = std::max<int64_t>(rows, 1);
-    const int64_t rp = round_up(rows, PACK_TAIL);
+    const int64_t rp = round_up(rows, PACK_ROWS);
     const int cg = rows > 128 ? 2 : 1;
     pl.ldk = (int)round_up(d, 8);
     pl.head = c.take<Head>(1);
@@ -598,9 +632,9 @@ constexpr int format_of() { return std::is_same<T, __half>::value ? 0 : 1; }
 
 // A kernel that may start while the one before it drains.
 template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*k)(P...), unsigned grid, unsigned block, cudaStream_t st, A... args) {
+cudaError_t launch_dependent(void (*k)(P...), dim3 grid, unsigned block, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -634,8 +668,8 @@ template <typename T>
 int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad) {
     const Pack p{a.hidden, a.ldh, a.targets, a.tb, (int)a.rows, (int)a.d, pl.ldk, a.vocab, lse, grad,
                  pl.head, pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat};
-    pack_rows_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, a.sms * 2), PACK_T, 0, a.st>>>(p);
-    MXS_TRY(cudaGetLastError());
+    MXS_TRY(launch_dependent(pack_rows_kernel<T>, (unsigned)std::min<int64_t>(ceil_div(a.rows, 4), a.sms * 4), PACK_T,
+                             a.st, p));
     return MXS_OK;
 }
 
@@ -652,7 +686,7 @@ int logit_tiles(LogitTiles<CG>& op, const Call& a, const Plan& pl, const void* w
     op.a_rows = CG == 1 ? (int)round_up(a.rows, 8) : 128;
     op.c = (float)(LOG2E / a.temperature);
     // rows of the tile that the box leaves out keep what shared memory held: their results are not read
-    if (!mxs::gemm::make_map(&op.mh, pl.packed, 2, a.d, round_up(a.rows, PACK_TAIL), pl.ldk, op.a_rows) ||
+    if (!mxs::gemm::make_map(&op.mh, pl.packed, 2, a.d, round_up(a.rows, PACK_ROWS), pl.ldk, op.a_rows) ||
         !mxs::gemm::make_map(&op.mw, w, 2, a.d, a.vocab, ldw, pl.n / CG))
         return MXS_ERR_CUDA;
     return MXS_OK;
@@ -669,8 +703,9 @@ int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss
     op.ytarget = pl.ytarget;
     const int64_t tiles = ceil_div(a.rows, 128 * CG) * pl.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
-    MXS_TRY(launch_dependent(score_join_kernel, (unsigned)ceil_div(a.rows, 8), 256, a.st, pl.part, pl.ytarget, pl.pos,
-                             (int)a.rows, pl.nt, loss, lse));
+    const bool whole = a.rows <= a.sms * 2;
+    MXS_TRY(launch_dependent(score_join_kernel, (unsigned)(whole ? a.rows : ceil_div(a.rows, 8)), 256, a.st, pl.part,
+                             pl.ytarget, pl.pos, (int)a.rows, pl.nt, whole, loss, lse));
     return MXS_OK;
 }
 
@@ -695,8 +730,8 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     prod.width = op.vocab;
     prod.first = v0 == 0;
     // columns after the piece are not read: the map ends there
-    if (!mxs::gemm::make_map(&prod.g_k, pl.g, 2, prod.width, round_up(a.rows, PACK_TAIL), pl.piece, 128) ||
-        !mxs::gemm::make_map(&prod.g_m, pl.g, 2, prod.width, round_up(a.rows, PACK_TAIL), pl.piece, 64))
+    if (!mxs::gemm::make_map(&prod.g_k, pl.g, 2, prod.width, round_up(a.rows, PACK_ROWS), pl.piece, 128) ||
+        !mxs::gemm::make_map(&prod.g_m, pl.g, 2, prod.width, round_up(a.rows, PACK_ROWS), pl.piece, 64))
         return MXS_ERR_CUDA;
     MXS_TRY(mxs::gemm::launch(prod, a.sms / 2, a.st));
     return MXS_OK;
@@ -743,16 +778,18 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
     prod.scale = (float)(1.0 / a.temperature / (format_of<T>() == 0 ? 16384.0 : 1.0));
     prod.vec = mxs::aligned16(gw, 2 * ldgw);
     if (!mxs::gemm::make_map(&prod.w_n, w, 2, a.d, a.vocab, ldw, 64) ||
-        !mxs::gemm::make_map(&prod.h_n, pl.packed, 2, a.d, round_up(a.rows, PACK_TAIL), pl.ldk, 64))
+        !mxs::gemm::make_map(&prod.h_n, pl.packed, 2, a.d, round_up(a.rows, PACK_ROWS), pl.ldk, 64))
         return MXS_ERR_CUDA;
     for (int64_t v0 = 0; v0 < a.vocab; v0 += pl.piece) {
         rc = a.rows > 128 ? grad_piece<2, T>(a, pl, w, ldw, v0, prod) : grad_piece<1, T>(a, pl, w, ldw, v0, prod);
         if (rc) return rc;
     }
-    if (gh)
-        MXS_TRY(launch_dependent(grad_hidden_out_kernel<T>, (unsigned)a.rows, 256, a.st, pl.acc, pl.pos, pl.head,
-                                 (int)a.d, pl.dn, (int)std::min(pl.piece, a.vocab), a.sms / 2, prod.scale,
-                                 static_cast<T*>(gh), ldgh));
+    for (int64_t r = 0; gh && r < a.rows; r += 65535) {  // as many rows as a grid counts
+        const dim3 grid((unsigned)ceil_div(a.d, 512), (unsigned)std::min<int64_t>(65535, a.rows - r));
+        MXS_TRY(launch_dependent(grad_hidden_out_kernel<T>, grid, 128, a.st, pl.acc, pl.pos + r, pl.head, (int)a.d,
+                                 pl.dn, (int)std::min(pl.piece, a.vocab), a.sms / 2, prod.scale,
+                                 static_cast<T*>(gh) + r * ldgh, ldgh));
+    }
     return MXS_OK;
 }
 
