@@ -49,18 +49,30 @@ struct Head {
 // Splits of K for `tiles` grad_hidden tiles: as many as fill the units, at least
 // 8 blocks of 64 columns each. A fixed function of the shape: the same sums in the same order every time.
 __host__ __device__ inline int grad_hidden_splits(int tiles, int width, int units) {
-    const int most = (width + 511) / 512;
-    const int s = tiles > 0 ? units / tiles : 1;
-    return s < 1 ? 1 : s < most ? s : most;
+    const int blocks = (width + 63) / 64, most = (blocks + 7) / 8;
+    int s = tiles > 0 ? units / tiles : 1;
+    s = s < 1 ? 1 : s < most ? s : most;
+    const int per = (blocks + s - 1) / s;
+    return (blocks + per - 1) / per;  // none of them empty
 }
+
+// The caller's targets: the row's, or -1 where it is outside the vocabulary.
+struct Targets {
+    const void* at;
+    int bytes;
+    int vocab;
+    __device__ __forceinline__ int operator()(int64_t r) const {
+        const int64_t t = bytes == 8 ? static_cast<const int64_t*>(at)[r]
+                                     : (int64_t)static_cast<const int32_t*>(at)[r];
+        return t >= 0 && t < vocab ? (int)t : -1;
+    }
+};
 
 struct Pack {
     const void* hidden;
     int64_t ld_hidden;
-    const void* targets;
-    int target_bytes;
+    Targets targets;
     int rows, d, ldk;
-    int64_t vocab;
     const float* lse;   // backward: null in forward
     const float* grad;
     Head* head;
@@ -70,15 +82,6 @@ struct Pack {
     float* lse2;        // [packed] lse * log2(e)
     float* ghat;        // [packed] grad / gmax
 };
-
-__device__ __forceinline__ int64_t target_of(const Pack& p, int64_t r) {
-    return p.target_bytes == 8 ? static_cast<const int64_t*>(p.targets)[r]
-                               : (int64_t)static_cast<const int32_t*>(p.targets)[r];
-}
-__device__ __forceinline__ bool kept_row(const Pack& p, int64_t r) {
-    const int64_t t = target_of(p, r);
-    return t >= 0 && t < p.vocab;
-}
 
 constexpr int PACK_T = 256;
 constexpr int PACK_ROWS = 256;  // packed rows are allocated in multiples of this
@@ -102,7 +105,7 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
     const int scan_to = p.grad ? p.rows : r0;
 #pragma unroll 4
     for (int r = tid; r < scan_to; r += PACK_T) {
-        const bool keep = kept_row(p, r);
+        const bool keep = p.targets(r) >= 0;
         const float g = p.grad ? fabsf(p.grad[r]) : 0.0f;
         all += keep;
         n += keep && r < r0;
@@ -129,7 +132,8 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
     const bool vec = reinterpret_cast<uintptr_t>(p.hidden) % 16 == 0 && p.ld_hidden % STEP == 0;
     for (int c0 = r0; c0 < r1; c0 += PACK_T) {
         const int r = c0 + tid;
-        const bool keep = r < r1 && kept_row(p, r);
+        const int tgt = r < r1 ? p.targets(r) : -1;
+        const bool keep = tgt >= 0;
         const uint32_t b = __ballot_sync(0xffffffffu, keep);
         __syncthreads();
         if (lane == 0) s_cnt[warp] = __popc(b);
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
         s_pos[tid] = keep ? at : -1;
         if (r < r1) p.pos[r] = keep ? at : -1;
         if (keep) {
-            p.target[at] = (int)target_of(p, r);
+            p.target[at] = tgt;
             if (p.grad) {
                 p.lse2[at] = p.lse[r] * (float)LOG2E;
                 p.ghat[at] = p.grad[r] / gm;
@@ -200,18 +204,37 @@ struct LogitTiles {
     int format;
     int64_t drop;
     uint32_t* status;
-    const Head* head;
+    const Head* head;    // null: the rows lie as the caller has them, none packed away
     const int* target;
+    Targets targets;     // read where the rows are not packed
     int rows, vocab;     // vocab: columns of this pass (its piece), starting at v0
     int v0, n, nt, kblocks, a_rows;
+    int span;            // CG 1: columns of a CTA
     float c;             // log2(e) / temperature
 
     __device__ void prefetch() const {
         mxs::gemm::prefetch_map(&mh);
         mxs::gemm::prefetch_map(&mw);
     }
-    __device__ int kept() const { return *(volatile const int*)&head->kept; }
+    __device__ int kept() const {
+        if (head) return *(volatile const int*)&head->kept;
+        return rows;  // not one conditional of two lvalues: that would load from either address
+    }
+    __device__ int target_of(int r) const {
+        if (head) return target[r];
+        return targets(r);
+    }
+    // CG 1 (one tile of rows): a CTA walks its own span of columns, so that all read
+    // the same amount of weight. CG 2: tiles go round the pairs.
     __device__ bool tile(int i, const Ctx& x, Tile& t) const {
+        if (CG == 1) {
+            const int64_t at = (int64_t)x.unit * span + (int64_t)i * n;
+            const int64_t end = min((int64_t)vocab, (int64_t)(x.unit + 1) * span);
+            if (at >= end || x.kept == 0) return false;
+            const int w = min(n, ((int)(end - at) + 31) / 32 * 32);
+            t = Tile{0, (int)at, 0, kblocks, w, x.unit * ((span + n - 1) / n) + i};
+            return true;
+        }
         const int mt = (x.kept + 128 * CG - 1) / (128 * CG);
         const int64_t idx = x.unit + (int64_t)i * x.units;
         if (idx >= (int64_t)mt * nt) return false;
@@ -221,10 +244,13 @@ struct LogitTiles {
     }
     __device__ bool a_mn(const Tile&) const { return false; }
     __device__ bool b_mn(const Tile&) const { return false; }
-    __device__ uint32_t bytes(const Tile&) const { return (uint32_t)(a_rows + n / CG) * 128; }
+    __device__ uint32_t bytes(const Tile& t) const { return (uint32_t)(a_rows + t.n / CG) * 128; }
     __device__ void load(const Tile& t, int kb, uint32_t sa, uint32_t sb, uint32_t bar, const Ctx& x) const {
         mxs::gemm::tma_load<CG>(sa, &mh, kb * 64, t.m0 + (int)x.rank * 128, bar);
-        mxs::gemm::tma_load<CG>(sb, &mw, kb * 64, v0 + t.n0 + (int)x.rank * (n / CG), bar);
+        if (CG == 1)  // boxes of 32 rows: a tile of any multiple of that
+            for (int j = 0; j < t.n; j += 32) mxs::gemm::tma_load<CG>(sb + j * 128, &mw, kb * 64, v0 + t.n0 + j, bar);
+        else
+            mxs::gemm::tma_load<CG>(sb, &mw, kb * 64, v0 + t.n0 + (int)x.rank * (n / CG), bar);
     }
     __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
 };
@@ -271,7 +297,7 @@ struct ScoreOp : LogitTiles<CG_> {
     __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx& x) const {
         const int r = t.m0 + me.row;
         if ((r & ~31) >= x.kept) return;  // the four warps of these rows agree
-        const int hit = r < x.kept ? this->target[r] - t.n0 : -1;  // the target's column of this tile
+        const int hit = r < x.kept ? this->target_of(r) - t.n0 : -1;  // the target's column of this tile
         const int cols = min(t.n, this->vocab - t.n0);
         float m = -INFINITY, s = 0.0f;
 #pragma unroll
@@ -329,14 +355,16 @@ __device__ __forceinline__ void join_pair(float& m, float& s, float om, float os
 // or (whole: few rows, where a warp's chain of reads would be most of the call)
 // a CTA.
 __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, const float* ytarget, const int* pos,
-                                                         int rows, int tiles, bool whole, float* loss, float* lse) {
+                                                         Targets targets, int rows, int tiles, bool whole,
+                                                         float* loss, float* lse) {
     __shared__ float2 s_pair[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = whole ? blockIdx.x : blockIdx.x * 8 + warp;
     mxs::gemm::grid_wait();
     mxs::gemm::grid_launch_dependents();
     if (r >= rows) return;
-    const int at = pos[r];
+    int at = targets(r) >= 0 ? r : -1;
+    if (pos) at = pos[r];
     if (at < 0) {
         if (whole ? threadIdx.x == 0 : lane == 0) {
             if (loss) loss[r] = 0.0f;
@@ -512,17 +540,12 @@ struct ProductOp {
         }
     }
     __device__ void zero(const Tile& t, const Lane& me, const Ctx&) const {
-        if (t.kind >= 0) {  // a split without columns
-            float* a = acc + ((int64_t)t.kind * 256 + me.row) * 256;
-            if (first)
-                for (int c0 = me.grp * 64; c0 < min(n, me.grp * 64 + 64); ++c0) a[c0] = 0.0f;
-            return;
-        }
-        const int m = t.m0 + me.row;
-        if (m >= width) return;
-        T* out = dw + (int64_t)(v0 + m) * lddw + t.n0;
-        for (int c0 = me.grp * 64; c0 < min(min(n, me.grp * 64 + 64), d - t.n0); ++c0)
-            out[c0] = mxs::from_f32<T>(0.0f);
+        if (t.kind >= 0) return;  // a split without columns, of a last piece: nothing to add
+        const int m = t.m0 + me.row - me.lane;
+        const float v[32] = {};
+        for (int c0 = me.grp * 32; c0 < n; c0 += 128)
+            mxs::gemm::store_rows<T, false>(dw + (int64_t)(v0 + m) * lddw + t.n0 + c0, lddw, v, width - m,
+                                            d - t.n0 - c0, vec, me);
     }
 };
 
@@ -582,10 +605,25 @@ struct Plan {
     void* w;          // the weight in aligned rows, if its own are not
     int ldk;
     int n, nt;        // logit tiles
+    int span;         // one tile of rows: columns of a CTA
+    bool direct;      // forward on the caller's own rows
     int dn, dnt;      // tiles over d_model
     int64_t piece;
     size_t bytes;
 };
+
+// Logit tiles over `cols` columns.
+void plan_tiles(Plan& pl, int sms, int64_t rows, int64_t cols) {
+    if (rows <= 128) {
+        pl.span = (int)round_up(ceil_div(cols, sms), 32);
+        pl.n = (int)round_up(ceil_div(pl.span, ceil_div(pl.span, 256)), 32);
+        const int64_t before = ceil_div(cols, pl.span) - 1;  // CTAs with a whole span
+        pl.nt = (int)(before * ceil_div(pl.span, pl.n) + ceil_div(cols - before * pl.span, pl.n));
+    } else {
+        pl.n = mxs::tile_width(ceil_div(rows, 256), cols, sms / 2, 64, 64);
+        pl.nt = (int)ceil_div(cols, pl.n);
+    }
+}
 
 Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows, int64_t d, int64_t vocab,
                bool backward) {
@@ -593,7 +631,6 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     Carve c(ws);
     rows = std::max<int64_t>(rows, 1);
     const int64_t rp = round_up(rows, PACK_ROWS);
-    const int cg = rows > 128 ? 2 : 1;
     pl.ldk = (int)round_up(d, 8);
     pl.head = c.take<Head>(1);
     pl.packed = c.take<uint16_t>((size_t)rp * pl.ldk);
@@ -601,8 +638,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     pl.target = c.take<int>(rows);
     pl.w = mxs::aligned16(weight, 2 * ldw) ? nullptr : c.take<uint16_t>((size_t)vocab * pl.ldk);
     if (!backward) {
-        pl.n = mxs::tile_width(ceil_div(rows, 128 * cg), vocab, sms / cg, 64, 32);
-        pl.nt = (int)ceil_div(vocab, pl.n);
+        plan_tiles(pl, sms, rows, vocab);
         pl.part = c.take<float2>((size_t)pl.nt * rows);
         pl.ytarget = c.take<float>(rows);
     } else {
@@ -610,7 +646,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
         pl.ghat = c.take<float>(rows);
         const int64_t most = std::max<int64_t>(256, PIECE_BYTES / (2 * rp));
         pl.piece = round_up(ceil_div(vocab, ceil_div(vocab, most)), 256);
-        pl.n = mxs::tile_width(ceil_div(rows, 128 * cg), pl.piece, sms / cg, 64, 64);
+        plan_tiles(pl, sms, rows, std::min(pl.piece, vocab));
         pl.g = c.take<uint16_t>((size_t)rp * pl.piece);
         pl.dn = d > 128 ? 256 : 128;
         pl.dnt = (int)ceil_div(d, pl.dn);
@@ -651,8 +687,7 @@ struct Call {
     const void* weight;
     int64_t ldw;
     int64_t rows, d, vocab;
-    const void* targets;
-    int tb;
+    Targets targets;
     double temperature;
     int sms;
     uint32_t* status;
@@ -666,8 +701,8 @@ struct Call {
 
 template <typename T>
 int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad) {
-    const Pack p{a.hidden, a.ldh, a.targets, a.tb, (int)a.rows, (int)a.d, pl.ldk, a.vocab, lse, grad,
-                 pl.head, pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat};
+    const Pack p{a.hidden, a.ldh, a.targets, (int)a.rows, (int)a.d, pl.ldk, lse, grad, pl.head,
+                 pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat};
     MXS_TRY(launch_dependent(pack_rows_kernel<T>, (unsigned)std::min<int64_t>(ceil_div(a.rows, 4), a.sms * 4), PACK_T,
                              a.st, p));
     return MXS_OK;
@@ -678,17 +713,20 @@ int logit_tiles(LogitTiles<CG>& op, const Call& a, const Plan& pl, const void* w
     op.format = format_of<T>();
     op.drop = mxs::test_drop_tile();
     op.status = a.status;
-    op.head = pl.head;
+    op.head = pl.direct ? nullptr : pl.head;
     op.target = pl.target;
+    op.targets = a.targets;
     op.rows = (int)a.rows;
     op.n = pl.n;
+    op.span = pl.span;
     op.kblocks = (int)ceil_div(a.d, 64);
     op.a_rows = CG == 1 ? (int)round_up(a.rows, 8) : 128;
     op.c = (float)(LOG2E / a.temperature);
     // rows of the tile that the box leaves out keep what shared memory held: their results are not read
-    if (!mxs::gemm::make_map(&op.mh, pl.packed, 2, a.d, round_up(a.rows, PACK_ROWS), pl.ldk, op.a_rows) ||
-        !mxs::gemm::make_map(&op.mw, w, 2, a.d, a.vocab, ldw, pl.n / CG))
-        return MXS_ERR_CUDA;
+    const bool rows_ok = pl.direct ? mxs::gemm::make_map(&op.mh, a.hidden, 2, a.d, a.rows, a.ldh, op.a_rows)
+                                   : mxs::gemm::make_map(&op.mh, pl.packed, 2, a.d, round_up(a.rows, PACK_ROWS), pl.ldk,
+                                                         op.a_rows);
+    if (!rows_ok || !mxs::gemm::make_map(&op.mw, w, 2, a.d, a.vocab, ldw, CG == 1 ? 32 : pl.n / 2)) return MXS_ERR_CUDA;
     return MXS_OK;
 }
 
@@ -701,11 +739,12 @@ int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss
     op.nt = pl.nt;
     op.part = pl.part;
     op.ytarget = pl.ytarget;
-    const int64_t tiles = ceil_div(a.rows, 128 * CG) * pl.nt;
-    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
+    const int64_t units = CG == 1 ? ceil_div(a.vocab, pl.span) : ceil_div(a.rows, 256) * pl.nt;
+    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
     const bool whole = a.rows <= a.sms * 2;
     MXS_TRY(launch_dependent(score_join_kernel, (unsigned)(whole ? a.rows : ceil_div(a.rows, 8)), 256, a.st, pl.part,
-                             pl.ytarget, pl.pos, (int)a.rows, pl.nt, whole, loss, lse));
+                             pl.ytarget, pl.direct ? nullptr : pl.pos, a.targets, (int)a.rows, pl.nt, whole, loss,
+                             lse));
     return MXS_OK;
 }
 
@@ -716,7 +755,7 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     if (rc) return rc;
     op.v0 = (int)v0;
     op.vocab = (int)std::min(pl.piece, a.vocab - v0);
-    op.nt = (int)ceil_div(op.vocab, pl.n);
+    op.nt = (int)ceil_div(op.vocab, pl.n);  // CG 2
     op.lse2 = pl.lse2;
     op.ghat = pl.ghat;
     op.g = static_cast<T*>(pl.g);
@@ -724,8 +763,8 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     // f16 holds G times 2^14: the target's entry stays below its largest value
     // and entries down to 2^-28 of the largest gradient weight stay normal numbers
     op.gscale = format_of<T>() == 0 ? 16384.0f : 1.0f;
-    const int64_t tiles = ceil_div(a.rows, 128 * CG) * op.nt;
-    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, tiles), a.st));
+    const int64_t units = CG == 1 ? ceil_div(op.vocab, pl.span) : ceil_div(a.rows, 256) * op.nt;
+    MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
     prod.v0 = (int)v0;
     prod.width = op.vocab;
     prod.first = v0 == 0;
@@ -738,15 +777,18 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
 }
 
 template <typename T>
-int forward(const Call& a, const Plan& pl, float* loss, float* lse) {
+int forward(const Call& a, Plan pl, float* loss, float* lse) {
     const void* w = a.weight;
     int64_t ldw = a.ldw;
     if (pl.w) {
         MXS_TRY(mxs::copy_rows(a.weight, 2 * a.ldw, pl.w, 2 * pl.ldk, a.vocab, 2 * a.d, a.sms, a.st));
         w = pl.w, ldw = pl.ldk;
     }
-    int rc = pack_rows<T>(a, pl, nullptr, nullptr);
-    if (rc) return rc;
+    // Up to 128 rows are one tile whether some are left out or not: where they are
+    // aligned they are read as they lie (rows left out compute numbers nobody reads).
+    pl.direct = a.rows <= 128 && mxs::aligned16(a.hidden, 2 * a.ldh);
+    if (!pl.direct)
+        if (const int rc = pack_rows<T>(a, pl, nullptr, nullptr)) return rc;
     return a.rows > 128 ? score<2, T>(a, pl, w, ldw, loss, lse) : score<1, T>(a, pl, w, ldw, loss, lse);
 }
 
@@ -817,8 +859,8 @@ int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const void* d_we
     if (bad_shape(ld_hidden, ld_weight, dtype, rows, d_model, vocab, target_bytes, temperature)) return MXS_ERR_INVALID;
     if (rows == 0) return MXS_OK;
     if (!d_hidden || !d_weight || !d_targets) return MXS_ERR_INVALID;
-    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab, d_targets, target_bytes, temperature, 0,
-           nullptr, static_cast<cudaStream_t>(stream)};
+    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab,
+           Targets{d_targets, target_bytes, (int)vocab}, temperature, 0, nullptr, static_cast<cudaStream_t>(stream)};
     const int rc = mxs::device_info(&a.sms, &a.status);
     if (rc) return rc;
     const Plan pl = make_plan(d_workspace, a.sms, d_weight, ld_weight, rows, d_model, vocab, false);
@@ -835,8 +877,8 @@ int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const v
         (d_grad_hidden && ld_grad_hidden < d_model) || (d_grad_weight && ld_grad_weight < d_model))
         return MXS_ERR_INVALID;
     if (!d_grad_hidden && !d_grad_weight) return MXS_OK;
-    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab, d_targets, target_bytes, temperature, 0,
-           nullptr, static_cast<cudaStream_t>(stream)};
+    Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab,
+           Targets{d_targets, target_bytes, (int)vocab}, temperature, 0, nullptr, static_cast<cudaStream_t>(stream)};
     if (rows == 0) {  // no row: the weight's gradient is zero
         if (d_grad_weight)
             MXS_TRY(cudaMemset2DAsync(d_grad_weight, 2 * ld_grad_weight, 0, 2 * d_model, vocab, a.st));

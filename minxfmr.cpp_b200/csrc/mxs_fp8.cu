@@ -279,6 +279,7 @@ struct MatmulOp {
     uint32_t* status;
     const float *sa, *sb;
     int rows, cols, kb, mt, nt, n, a_rows;
+    int span;  // CG 1: columns of a CTA
     O* out;
     int64_t ldo;
     bool vec;
@@ -288,19 +289,31 @@ struct MatmulOp {
         mxs::gemm::prefetch_map(&mb);
     }
     __device__ int kept() const { return rows; }
+    // CG 1 (one tile of rows): a CTA walks its own span of columns, so that all read
+    // the same amount of b. CG 2: tiles go round the pairs, rows fastest.
     __device__ bool tile(int i, const Ctx& x, Tile& t) const {
+        if (CG == 1) {
+            const int64_t at = (int64_t)x.unit * span + (int64_t)i * n;
+            const int64_t end = min((int64_t)cols, (int64_t)(x.unit + 1) * span);
+            if (at >= end) return false;
+            t = Tile{0, (int)at, 0, kb, min(n, ((int)(end - at) + 31) / 32 * 32), 0};
+            return true;
+        }
         const int64_t idx = x.unit + (int64_t)i * x.units;
         if (idx >= (int64_t)mt * nt) return false;
         const int m = (int)(idx % mt), v = (int)(idx / mt);
-        t = Tile{m * 128 * CG, v * n, 0, kb, n, v};
+        t = Tile{m * 128 * CG, v * n, 0, kb, n, 0};
         return true;
     }
     __device__ bool a_mn(const Tile&) const { return false; }
     __device__ bool b_mn(const Tile&) const { return false; }
-    __device__ uint32_t bytes(const Tile&) const { return (uint32_t)(a_rows + n / CG) * 128; }
+    __device__ uint32_t bytes(const Tile& t) const { return (uint32_t)(a_rows + t.n / CG) * 128; }
     __device__ void load(const Tile& t, int k, uint32_t s_a, uint32_t s_b, uint32_t bar, const Ctx& x) const {
         mxs::gemm::tma_load<CG>(s_a, &ma, k * BLK, t.m0 + (int)x.rank * 128, bar);
-        mxs::gemm::tma_load<CG>(s_b, &mb, k * BLK, t.n0 + (int)x.rank * (n / CG), bar);
+        if (CG == 1)  // boxes of 32 rows: a tile of any multiple of that
+            for (int j = 0; j < t.n; j += 32) mxs::gemm::tma_load<CG>(s_b + j * 128, &mb, k * BLK, t.n0 + j, bar);
+        else
+            mxs::gemm::tma_load<CG>(s_b, &mb, k * BLK, t.n0 + (int)x.rank * (n / CG), bar);
     }
     __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
     __device__ void fetch(Acc& a, int k) const {
@@ -358,7 +371,7 @@ struct MatmulOp {
 
 template <int CG, typename O, int RUNS>
 int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
-                 int64_t n, int64_t k, void* out, int64_t ldo, int width, int sms, uint32_t* status, cudaStream_t st) {
+                 int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status, cudaStream_t st) {
     MatmulOp<CG, O, RUNS> op{};
     op.format = 0;
     op.drop = mxs::test_drop_tile();
@@ -367,25 +380,27 @@ int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int
     op.rows = (int)rows, op.cols = (int)n, op.kb = (int)ceil_div(k, BLK);
     op.mt = (int)ceil_div(rows, 128 * CG);
     op.n = width;
+    op.span = span;
     op.nt = (int)ceil_div(n, op.n);
     op.a_rows = CG == 1 ? (int)round_up(rows, 8) : 128;
     op.out = static_cast<O*>(out);
     op.ldo = ldo;
     op.vec = mxs::aligned16(out, ldo * (int64_t)sizeof(O));
     if (!mxs::gemm::make_map(&op.ma, a, 1, k, rows, lda, op.a_rows) ||
-        !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, op.n / CG))
+        !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, CG == 1 ? 32 : op.n / 2))
         return MXS_ERR_CUDA;
-    const int64_t tiles = (int64_t)op.mt * op.nt;
-    return mxs::gemm::launch(op, (int)std::min<int64_t>(sms / CG, tiles), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+    const int64_t units = CG == 1 ? ceil_div(n, span) : (int64_t)op.mt * op.nt;
+    return mxs::gemm::launch(op, (int)std::min<int64_t>(sms / CG, units), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
 }
 
 template <typename O>
 int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
                   int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
-    const int cg = rows > 128 ? 2 : 1;
-    const int w = mxs::tile_width(ceil_div(rows, 128 * cg), n, sms / cg, 64, 32);
-    auto go = [&](auto f) { return f(a, lda, sa, b, ldb, sb, rows, n, k, out, ldo, w, sms, status, st); };
-    if (cg == 2) return w > 128 ? go(launch_tiles<2, O, 4>) : go(launch_tiles<2, O, 2>);
+    const int span = (int)round_up(ceil_div(n, sms), 32);  // up to 128 rows: one tile of them
+    const int w = rows > 128 ? mxs::tile_width(ceil_div(rows, 256), n, sms / 2, 64, 32)
+                             : (int)round_up(ceil_div(span, ceil_div(span, 256)), 32);
+    auto go = [&](auto f) { return f(a, lda, sa, b, ldb, sb, rows, n, k, out, ldo, w, span, sms, status, st); };
+    if (rows > 128) return w > 128 ? go(launch_tiles<2, O, 4>) : go(launch_tiles<2, O, 2>);
     return w > 128 ? go(launch_tiles<1, O, 4>) : go(launch_tiles<1, O, 2>);
 }
 

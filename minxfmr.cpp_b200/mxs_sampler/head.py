@@ -68,7 +68,7 @@ def _vector(t, n, name, dtypes):
 def _scratch(query, args, dev):
     n = ctypes.c_size_t()
     _check(query, getattr(load(), query)(*args, ctypes.byref(n)))
-    return torch.empty(max(n.value, 1), dtype=torch.uint8, device=dev)
+    return torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
 
 
 def _same_device(dev, **tensors):
@@ -106,7 +106,7 @@ def ce_from_hidden(hidden, weight, targets, temperature=1.0, stream=None):
         lse = torch.empty(rows, dtype=torch.float32, device=dev)
         ws = _scratch("mxs_ce_workspace_size", (_ptr(weight), ldw, rows, d, vocab, 0), dev)
         rc = load().mxs_ce_from_hidden(_ptr(hidden), ldh, _ptr(weight), ldw, dt, rows, d, vocab, _ptr(targets), tb,
-                                       float(temperature), _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(),
+                                       float(temperature), _ptr(loss), _ptr(lse), _ptr(ws), ws.numel() if ws is not None else 0,
                                        _stream(stream, dev))
     _check("mxs_ce_from_hidden", rc)
     return loss, lse
@@ -128,7 +128,7 @@ def ce_from_hidden_backward(hidden, weight, targets, lse, grad_loss, temperature
         ws = _scratch("mxs_ce_workspace_size", (_ptr(weight), ldw, rows, d, vocab, 1), dev)
         rc = load().mxs_ce_from_hidden_backward(_ptr(hidden), ldh, _ptr(weight), ldw, dt, rows, d, vocab,
                                                 _ptr(targets), tb, float(temperature), _ptr(lse), _ptr(grad_loss),
-                                                _ptr(gh), d, _ptr(gw), d, _ptr(ws), ws.numel(), _stream(stream, dev))
+                                                _ptr(gh), d, _ptr(gw), d, _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream, dev))
     _check("mxs_ce_from_hidden_backward", rc)
     return gh, gw
 
@@ -209,7 +209,7 @@ def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.float32, out=None, stream
         ldo = _matrix(out, "out")
         ws = _scratch("mxs_matmul_fp8_workspace_size", (_ptr(a), lda, _ptr(b), ldb, rows, n, k), dev)
         rc = load().mxs_matmul_fp8(_ptr(a), lda, _ptr(a_scale), _ptr(b), ldb, _ptr(b_scale), rows, n, k, _ptr(out),
-                                   ldo, _CODES[out.dtype], _ptr(ws), ws.numel(), _stream(stream, dev))
+                                   ldo, _CODES[out.dtype], _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream, dev))
     _check("mxs_matmul_fp8", rc)
     return out
 
@@ -243,6 +243,6 @@ def sample_from_hidden_fp8(hidden, weight_q, weight_scale, temperature, top_k, u
         rc = load().mxs_sample_from_hidden_fp8(_ptr(hidden), ldh, dt, _ptr(weight_q), ldw, _ptr(weight_scale), rows, d,
                                                vocab, float(temperature), int(top_k), float(top_p), float(min_p),
                                                _ptr(u), _ptr(nxt), _ptr(idx), _ptr(prob), _ptr(logits_out), ldl,
-                                               _ptr(ws), ws.numel(), _stream(stream, dev))
+                                               _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream, dev))
     _check("mxs_sample_from_hidden_fp8", rc)
     return nxt, idx, prob
