@@ -336,7 +336,7 @@ struct ScoreOp : LogitTiles<CG_> {
         if (me.grp != 0 || r >= x.kept) return;
 #pragma unroll
         for (int g = 1; g < 4; ++g) {  // group g's warp is four places on
-            const float2 q = mine[g * 4 * (mxs::gemm::XPOSE / 8)];
+            const float2 q = mine[g * 4 * (mxs::gemm::XPOSE_ALL / LogitTiles<CG_>::EPI / 8)];
             const float nm = fmaxf(m, q.x), sub = nm == -INFINITY ? 0.0f : nm;
             s = s * ex2(m - sub) + q.y * ex2(q.x - sub);
             m = nm;

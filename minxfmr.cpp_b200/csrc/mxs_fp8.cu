@@ -264,7 +264,7 @@ cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
 template <int CG_, typename O, int RUNS>
 struct MatmulOp {
     static constexpr int CG = CG_;
-    static constexpr int EPI = 8;
+    static constexpr int EPI = 8, STEP = 8 * EPI;  // columns from one run of a thread to its next
     static constexpr bool F8 = true, PROMOTE = true;
     __device__ int group() const { return 1; }
     struct Acc {
@@ -327,7 +327,7 @@ struct MatmulOp {
         a.ra = sa + (int64_t)min(rows - 1, t.m0 + me.row) * kb;
 #pragma unroll
         for (int i = 0; i < RUNS; ++i)  // 32 columns lie in one block of 128
-            a.rb[i] = sb + (int64_t)(min(cols - 1, t.n0 + me.grp * 32 + i * 64) / BLK) * kb;
+            a.rb[i] = sb + (int64_t)(min(cols - 1, t.n0 + me.grp * 32 + i * STEP) / BLK) * kb;
         fetch(a, 0);
     }
     __device__ void prepare(Acc& a, const Tile&, int k, const Lane&, const Ctx&) const {
@@ -337,24 +337,15 @@ struct MatmulOp {
     }
     template <typename Release>
     __device__ void join(Acc& a, const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, Release release) const {
-        // the next run is on its way while one is joined; a run past the tile's is not kept
         const int c0 = me.grp * 32, end = t.n - 32;
-        float x[32], y[32];
-        auto add = [&](int i, const float (&p)[32]) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(p[j], a.now[i], a.v[i][j]);
-        };
-        mxs::gemm::tmem_ld32(tmem + min(c0, end), x);
-        mxs::gemm::tmem_ld32(tmem + min(c0 + 64, end), y);
-        if (RUNS == 4) {
-            add(0, x);
-            mxs::gemm::tmem_ld32(tmem + min(c0 + 128, end), x);
-            add(1, y);
-            mxs::gemm::tmem_ld32(tmem + min(c0 + 192, end), y);
+        for (int i = 0; i < RUNS; ++i) {
+            float x[32];
+            mxs::gemm::tmem_ld32(tmem + min(c0 + i * STEP, end), x);  // a run past the tile's is not kept
+            if (i == RUNS - 1) release();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(x[j], a.now[i], a.v[i][j]);
         }
-        release();
-        add(RUNS - 2, x);
-        add(RUNS - 1, y);
     }
     __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
         const int r0 = t.m0 + me.row - me.lane;
@@ -362,9 +353,9 @@ struct MatmulOp {
         O* o = out + (int64_t)r0 * ldo + t.n0;
 #pragma unroll
         for (int i = 0; i < RUNS; ++i) {
-            const int c0 = me.grp * 32 + i * 64;
+            const int c0 = me.grp * 32 + i * STEP;
             if (c0 >= t.n) break;
-            mxs::gemm::store_rows<O, false>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
+            mxs::gemm::store_rows<O, false, 32 * sizeof(O)>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
         }
     }
 };

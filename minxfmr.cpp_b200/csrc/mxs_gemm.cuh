@@ -43,17 +43,18 @@ namespace gemm {
 
 constexpr int EPI_WARP0 = 4;
 constexpr int MAX_ACC = 8;  // accumulators that TMEM holds at most
-constexpr int XPOSE = 2048;  // bytes of shared memory for each epilogue warp's transposes
+constexpr int XPOSE_ALL = 32768;  // shared memory for the epilogue warps' transposes
 constexpr int A_BYTES = 128 * 128;
 constexpr int ROW = 128;  // bytes of a stage row (one swizzle row)
 
 template <typename Op>
 struct Geo {
     static constexpr int CG = Op::CG, THREADS = 32 * (EPI_WARP0 + Op::EPI);
+    static constexpr int XPOSE = XPOSE_ALL / Op::EPI;  // of one warp: 2 or 4 KB
     static constexpr int B_BYTES = 256 / CG * ROW;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = 196608 / STAGE;  // 192 KB: 4 or 6
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + Op::EPI * XPOSE + 512;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + XPOSE_ALL + 512;
 };
 
 struct Tile {
@@ -68,7 +69,7 @@ struct Tile {
 struct Lane {
     int lane, quad, grp;  // quad: which 32 rows of the CTA's 128; grp: which column group
     int row;              // of the pair's tile
-    uint8_t* xpose;       // its warp's XPOSE bytes
+    uint8_t* xpose;       // its warp's bytes for transposes
 };
 
 struct Ring {
@@ -189,26 +190,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// The same as pairs of floats in 64-bit registers, for the paired multiply-add:
-// made inside the block, the pairs are the loaded registers themselves, without
-// moves. (The wait costs nothing here: the values' first use waits.)
-__device__ __forceinline__ void tmem_ld32_pairs(uint32_t addr, uint64_t (&p)[16]) {
-    asm volatile(
-        "{\n .reg .b32 t<32>;\n"
-        " tcgen05.ld.sync.aligned.32x32b.x32.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15,"
-        " t16, t17, t18, t19, t20, t21, t22, t23, t24, t25, t26, t27, t28, t29, t30, t31}, [%16];\n"
-        " tcgen05.wait::ld.sync.aligned;\n"
-        " mov.b64 %0, {t0, t1}; mov.b64 %1, {t2, t3}; mov.b64 %2, {t4, t5}; mov.b64 %3, {t6, t7};\n"
-        " mov.b64 %4, {t8, t9}; mov.b64 %5, {t10, t11}; mov.b64 %6, {t12, t13}; mov.b64 %7, {t14, t15};\n"
-        " mov.b64 %8, {t16, t17}; mov.b64 %9, {t18, t19}; mov.b64 %10, {t20, t21}; mov.b64 %11, {t22, t23};\n"
-        " mov.b64 %12, {t24, t25}; mov.b64 %13, {t26, t27}; mov.b64 %14, {t28, t29}; mov.b64 %15, {t30, t31};\n"
-        "}"
-        : "=l"(p[0]), "=l"(p[1]), "=l"(p[2]), "=l"(p[3]), "=l"(p[4]), "=l"(p[5]), "=l"(p[6]), "=l"(p[7]),
-          "=l"(p[8]), "=l"(p[9]), "=l"(p[10]), "=l"(p[11]), "=l"(p[12]), "=l"(p[13]), "=l"(p[14]), "=l"(p[15])
-        : "r"(addr)
-        : "memory");
-}
-
 // Whether the unrolled j is the value h, kept as a comparison (the compiler would
 // turn the run of them into an index, and the array into local memory).
 __device__ __forceinline__ bool is_column(int h, int j) {
@@ -217,60 +198,52 @@ __device__ __forceinline__ bool is_column(int h, int j) {
     return d == 0;
 }
 
-// Pairs of floats in 64-bit registers.
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
-    return p;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
-}
-__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) {  // c += a * b
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
-}
-
-// A warp's 32 x 32 values (a row a thread) to row-major memory, through its
-// XPOSE bytes: a store from the threads' own rows touches 32 lines for 16 bytes
-// each, one from here 8 rows of 64 bytes. `out` is the place of row 0, column 0;
-// `rows` and `cols` say how many of the 32 exist; `vec` that rows start on 16-byte
-// boundaries. ADD adds to what is there.
-template <typename T, bool ADD>
+// A warp's 32 x 32 values (a row a thread) to row-major memory, through its share
+// of shared memory, LINE bytes of a row at a time (64 or 128: 32 rows of it must
+// fit): a store from the threads' own rows touches 32 lines for 16 bytes each, one
+// from here 4 or 8 lines. `out` is the place of row 0, column 0; `rows` and `cols`
+// say how many of the 32 exist; `vec` that rows start on 16-byte boundaries. ADD
+// adds to what is there.
+template <typename T, bool ADD, int LINE = 64>
 __device__ __forceinline__ void store_rows(T* out, int64_t ld, const float (&v)[32], int rows, int cols, bool vec,
                                            const Lane& me) {
-    constexpr int EACH = 16 / sizeof(T);  // values of a 16-byte piece; a pass takes four pieces of a row
-    constexpr int W = 4 * EACH;
-    const int l = me.lane;
+    constexpr int EACH = 16 / sizeof(T);                  // values of a 16-byte piece
+    constexpr int W = LINE / (int)sizeof(T);              // values of a line
+    constexpr int PIECES = LINE / 16, SHIFT = LINE == 64 ? 1 : 0;  // a row's pieces, in an order of its own:
+    const int l = me.lane;                                // neighbouring rows' fall into different banks
+    auto slot = [&](int r, int p) { return me.xpose + r * LINE + ((p ^ (r >> SHIFT)) & (PIECES - 1)) * 16; };
 #pragma unroll
     for (int c0 = 0; c0 < 32; c0 += W) {
         __syncwarp();
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-            *reinterpret_cast<uint4*>(me.xpose + l * 64 + ((p ^ (l >> 1)) & 3) * 16) = pack16<T>(v + c0 + p * EACH);
+        for (int p = 0; p < PIECES; ++p) *reinterpret_cast<uint4*>(slot(l, p)) = pack16<T>(v + c0 + p * EACH);
         __syncwarp();
         if (vec && cols >= c0 + W) {
+            constexpr int STEP = 32 / PIECES;  // rows of one store
+            uint4 u[PIECES];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int r = p * 8 + (l >> 2);
-                uint4 u = *reinterpret_cast<const uint4*>(me.xpose + r * 64 + (((l & 3) ^ (r >> 1)) & 3) * 16);
+            for (int p = 0; p < PIECES; ++p)
+                u[p] = *reinterpret_cast<const uint4*>(slot(p * STEP + l / PIECES, l % PIECES));
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const int r = p * STEP + l / PIECES;
                 if (r >= rows) continue;
-                uint4* to = reinterpret_cast<uint4*>(out + (int64_t)r * ld + c0 + (l & 3) * EACH);
+                uint4* to = reinterpret_cast<uint4*>(out + (int64_t)r * ld + c0 + (l % PIECES) * EACH);
                 if (ADD) {
                     const uint4 o = *to;
-                    u.x = __float_as_uint(__uint_as_float(u.x) + __uint_as_float(o.x));
-                    u.y = __float_as_uint(__uint_as_float(u.y) + __uint_as_float(o.y));
-                    u.z = __float_as_uint(__uint_as_float(u.z) + __uint_as_float(o.z));
-                    u.w = __float_as_uint(__uint_as_float(u.w) + __uint_as_float(o.w));
+                    u[p].x = __float_as_uint(__uint_as_float(u[p].x) + __uint_as_float(o.x));
+                    u[p].y = __float_as_uint(__uint_as_float(u[p].y) + __uint_as_float(o.y));
+                    u[p].z = __float_as_uint(__uint_as_float(u[p].z) + __uint_as_float(o.z));
+                    u[p].w = __float_as_uint(__uint_as_float(u[p].w) + __uint_as_float(o.w));
                 }
-                *to = u;
+                *to = u[p];
             }
         } else {
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const int r = i * (32 / W) + l / W, c = l % W;
                 if (r < rows && c0 + c < cols)
-                    out[(int64_t)r * ld + c0 + c] = reinterpret_cast<const T*>(
-                        me.xpose + r * 64 + (((c / EACH) ^ (r >> 1)) & 3) * 16)[c % EACH];
+                    out[(int64_t)r * ld + c0 + c] = reinterpret_cast<const T*>(slot(r, c / EACH))[c % EACH];
             }
         }
     }
@@ -347,7 +320,7 @@ __device__ __forceinline__ void run(const Op& op) {
     extern __shared__ uint8_t raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* xpose = base + (size_t)G::STAGES * G::STAGE;
-    Ring* ring = reinterpret_cast<Ring*>(xpose + Op::EPI * XPOSE);
+    Ring* ring = reinterpret_cast<Ring*>(xpose + XPOSE_ALL);
     const uint32_t stages = smem_u32(base);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Ctx ctx;
@@ -431,7 +404,9 @@ __device__ __forceinline__ void run(const Op& op) {
                 const int group = op.group() < t.kn ? op.group() : t.kn;
                 int in = 0;  // block of its group
                 for (int kb = 0; kb < t.kn; ++kb) {
-                    ok = (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring)) && wait(&ring->full[s], ph, ring);
+                    // the operands first: they are there long before an accumulator comes free, and
+                    // a wait costs 100 clocks even where it has nothing to wait for
+                    ok = wait(&ring->full[s], ph, ring) && (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring));
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     fence_after();
                     const bool last = in + 1 == group || kb == t.kn - 1;
@@ -469,7 +444,7 @@ __device__ __forceinline__ void run(const Op& op) {
         me.quad = warp & 3;
         me.grp = (warp - EPI_WARP0) >> 2;
         me.row = (int)ctx.rank * 128 + me.quad * 32 + lane;
-        me.xpose = xpose + (warp - EPI_WARP0) * XPOSE;
+        me.xpose = xpose + (warp - EPI_WARP0) * G::XPOSE;
         const uint32_t lanes = (uint32_t)(me.quad * 32) << 16;
         const uint32_t te0 = CG == 2 ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
         uint32_t buf = 0, tph = 0;
