@@ -197,7 +197,7 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, 2^-22 relative; results
 template <int CG_>
 struct LogitTiles {
     static constexpr int CG = CG_;
-    static constexpr int EPI = 16;
+    static constexpr int EPI = 16, SWAP = 0;
     static constexpr bool F8 = false, PROMOTE = false;
     __device__ int group() const { return INT32_MAX; }
     CUtensorMap mh, mw;
@@ -445,7 +445,7 @@ struct GradLogitsOp : LogitTiles<CG_> {
 template <typename T>
 struct ProductOp {
     static constexpr int CG = 2;
-    static constexpr int EPI = 16;
+    static constexpr int EPI = 16, SWAP = 0;
     static constexpr bool F8 = false, PROMOTE = false;
     __device__ int group() const { return INT32_MAX; }
     CUtensorMap g_k, g_m, w_n, h_n;

@@ -258,13 +258,23 @@ cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
 // 256 of accumulator reads and 256 of FMA a scheduler).
 // ---------------------------------------------------------------------------
 
+// The i-th tile of a CTA that walks its own `span` of the columns, n at a time, so
+// that all CTAs read the same amount of the second operand.
+__device__ __forceinline__ bool span_tile(int i, const Ctx& x, int span, int n, int cols, int kb, Tile& t) {
+    const int64_t at = (int64_t)x.unit * span + (int64_t)i * n;
+    const int64_t end = min((int64_t)cols, (int64_t)(x.unit + 1) * span);
+    if (at >= end) return false;
+    t = Tile{0, (int)at, 0, kb, min(n, ((int)(end - at) + 31) / 32 * 32), 0};
+    return true;
+}
+
 // RUNS: runs of 32 columns a thread holds, 4 for tiles of up to 256 columns, 2 for
 // up to 128. The join has no branch around the sums (a warp without rows joins what
 // it finds and stores nothing): where two paths meet the compiler copies all 128.
 template <int CG_, typename O, int RUNS>
 struct MatmulOp {
     static constexpr int CG = CG_;
-    static constexpr int EPI = 8, STEP = 8 * EPI;  // columns from one run of a thread to its next
+    static constexpr int EPI = 8, SWAP = 0, STEP = 8 * EPI;  // columns from one run of a thread to its next
     static constexpr bool F8 = true, PROMOTE = true;
     __device__ int group() const { return 1; }
     struct Acc {
@@ -289,16 +299,9 @@ struct MatmulOp {
         mxs::gemm::prefetch_map(&mb);
     }
     __device__ int kept() const { return rows; }
-    // CG 1 (one tile of rows): a CTA walks its own span of columns, so that all read
-    // the same amount of b. CG 2: tiles go round the pairs, rows fastest.
+    // CG 1 (one tile of rows): spans. CG 2: tiles go round the pairs, rows fastest.
     __device__ bool tile(int i, const Ctx& x, Tile& t) const {
-        if (CG == 1) {
-            const int64_t at = (int64_t)x.unit * span + (int64_t)i * n;
-            const int64_t end = min((int64_t)cols, (int64_t)(x.unit + 1) * span);
-            if (at >= end) return false;
-            t = Tile{0, (int)at, 0, kb, min(n, ((int)(end - at) + 31) / 32 * 32), 0};
-            return true;
-        }
+        if (CG == 1) return span_tile(i, x, span, n, cols, kb, t);
         const int64_t idx = x.unit + (int64_t)i * x.units;
         if (idx >= (int64_t)mt * nt) return false;
         const int m = (int)(idx % mt), v = (int)(idx / mt);
@@ -360,6 +363,99 @@ struct MatmulOp {
     }
 };
 
+// Up to 64 rows, as a decode step has them: the weight's rows lie along TMEM's
+// lanes, 128 at a time, and NP >= rows rows of a along its columns. A thread holds
+// one weight row's sums for NP rows, so the join costs what the rows there are
+// cost, not 128, and the tensor core reads 4 KB of weight and NP * 32 bytes of a
+// for 128 weight rows (operand reads, 64 bytes a clock, are what bounds an MMA of
+// one CTA). Stores are 32 neighbouring columns a warp, whatever their alignment.
+// Bound by the weight's bytes.
+template <typename O, int NP>
+struct DecodeOp {
+    static constexpr int CG = 1, EPI = 8, SWAP = NP;
+    static constexpr bool F8 = true, PROMOTE = true;
+    __device__ int group() const { return 1; }
+    struct Acc {
+        float v[NP];
+        const float *ra[NP > 32 ? 2 : 1], *rb;  // scales of rows lane, lane + 32 of a; of the warp's weight rows
+        float next_a[NP > 32 ? 2 : 1], next_b;
+    };
+    CUtensorMap ma, mb;
+    int format;
+    int64_t drop;
+    uint32_t* status;
+    const float *sa, *sb;
+    int rows, cols, kb, n, a_rows, span;
+    O* out;
+    int64_t ldo;
+
+    __device__ void prefetch() const {
+        mxs::gemm::prefetch_map(&ma);
+        mxs::gemm::prefetch_map(&mb);
+    }
+    __device__ int kept() const { return rows; }
+    __device__ bool tile(int i, const Ctx& x, Tile& t) const { return span_tile(i, x, span, n, cols, kb, t); }
+    __device__ bool a_mn(const Tile&) const { return false; }
+    __device__ bool b_mn(const Tile&) const { return false; }
+    __device__ uint32_t bytes(const Tile& t) const { return (uint32_t)(a_rows + t.n) * 128; }
+    __device__ void load(const Tile& t, int k, uint32_t s_a, uint32_t s_b, uint32_t bar, const Ctx&) const {
+        mxs::gemm::tma_load<CG>(s_a, &ma, k * BLK, 0, bar);
+        for (int j = 0; j < t.n; j += 32) mxs::gemm::tma_load<CG>(s_b + j * 128, &mb, k * BLK, t.n0 + j, bar);
+    }
+    __device__ void zero(const Tile&, const Lane&, const Ctx&) const {}
+    // first weight row of the warp, of the tile's
+    __device__ int first(const Lane& me) const { return me.grp * 128 + me.quad * 32; }
+    __device__ void fetch(Acc& a, int k) const {
+#pragma unroll
+        for (int i = 0; i < (NP > 32 ? 2 : 1); ++i) a.next_a[i] = a.ra[i][k];
+        a.next_b = a.rb[k];
+    }
+    __device__ void begin(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) a.v[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < (NP > 32 ? 2 : 1); ++i) a.ra[i] = sa + (int64_t)min(rows - 1, me.lane + 32 * i) * kb;
+        a.rb = sb + (int64_t)(min(cols - 1, t.n0 + first(me)) / BLK) * kb;  // 32 weight rows lie in one block of 128
+        fetch(a, 0);
+    }
+    // the rows' scales of the block, times the weight's, where every lane can read them
+    __device__ void prepare(Acc& a, const Tile&, int k, const Lane& me, const Ctx&) const {
+        float* s = reinterpret_cast<float*>(me.xpose);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < (NP > 32 ? 2 : 1); ++i) s[me.lane + 32 * i] = a.next_a[i] * a.next_b;
+        __syncwarp();
+        fetch(a, min(k + 1, kb - 1));
+    }
+    template <typename Release>
+    __device__ void join(Acc& a, const Tile&, uint32_t tmem, const Lane& me, const Ctx&, Release release) const {
+        const float4* s = reinterpret_cast<const float4*>(me.xpose);
+        constexpr int W = NP < 32 ? NP : 32;
+#pragma unroll
+        for (int i = 0; i < NP; i += W) {
+            float x[W];
+            mxs::gemm::tmem_ld(tmem + me.grp * NP + i, x);
+            if (i + W == NP) release();
+#pragma unroll
+            for (int j = 0; j < W; j += 4) {
+                const float4 q = s[(i + j) / 4];
+                a.v[i + j] = fmaf(x[j], q.x, a.v[i + j]);
+                a.v[i + j + 1] = fmaf(x[j + 1], q.y, a.v[i + j + 1]);
+                a.v[i + j + 2] = fmaf(x[j + 2], q.z, a.v[i + j + 2]);
+                a.v[i + j + 3] = fmaf(x[j + 3], q.w, a.v[i + j + 3]);
+            }
+        }
+    }
+    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
+        const int c = first(me) + me.lane;
+        if (c >= t.n || t.n0 + c >= cols) return;
+        O* o = out + t.n0 + c;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+            if (i < rows) o[(int64_t)i * ldo] = mxs::from_f32<O>(a.v[i]);
+    }
+};
+
 template <int CG, typename O, int RUNS>
 int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
                  int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status, cudaStream_t st) {
@@ -384,6 +480,26 @@ int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int
     return mxs::gemm::launch(op, (int)std::min<int64_t>(sms / CG, units), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
 }
 
+template <typename O, int NP>
+int launch_decode(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
+                  int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status,
+                  cudaStream_t st) {
+    DecodeOp<O, NP> op{};
+    op.format = 0;
+    op.drop = mxs::test_drop_tile();
+    op.status = status;
+    op.sa = sa, op.sb = sb;
+    op.rows = (int)rows, op.cols = (int)n, op.kb = (int)ceil_div(k, BLK);
+    op.n = width;
+    op.span = span;
+    op.a_rows = (int)round_up(rows, 8);  // rows that the box leaves out give columns nobody reads
+    op.out = static_cast<O*>(out);
+    op.ldo = ldo;
+    if (!mxs::gemm::make_map(&op.ma, a, 1, k, rows, lda, op.a_rows) || !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, 32))
+        return MXS_ERR_CUDA;
+    return mxs::gemm::launch(op, (int)ceil_div(n, span), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
+}
+
 template <typename O>
 int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
                   int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
@@ -391,6 +507,10 @@ int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, in
     const int w = rows > 128 ? mxs::tile_width(ceil_div(rows, 256), n, sms / 2, 64, 32)
                              : (int)round_up(ceil_div(span, ceil_div(span, 256)), 32);
     auto go = [&](auto f) { return f(a, lda, sa, b, ldb, sb, rows, n, k, out, ldo, w, span, sms, status, st); };
+    // Rows along the columns up to 64 of them; 128 rows' sums no longer fit a thread beside the loads.
+    if (rows <= 16) return go(launch_decode<O, 16>);
+    if (rows <= 32) return go(launch_decode<O, 32>);
+    if (rows <= 64) return go(launch_decode<O, 64>);
     if (rows > 128) return w > 128 ? go(launch_tiles<2, O, 4>) : go(launch_tiles<2, O, 2>);
     return w > 128 ? go(launch_tiles<1, O, 4>) : go(launch_tiles<1, O, 2>);
 }

@@ -190,6 +190,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[32]) { tmem_ld32(addr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15},"
+        " [%16];\n tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // Whether the unrolled j is the value h, kept as a comparison (the compiler would
 // turn the run of them into an index, and the array into local memory).
 __device__ __forceinline__ bool is_column(int h, int j) {
@@ -285,8 +299,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ring* ring)
 // is TMEM, ordered by the tcgen05 fences; no memory is published, so the arrival
 // is relaxed (a release for the cluster waits for every load and store in flight:
 // 1000 to 2000 clocks for each block of the 8-bit product).
-__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+__device__ __forceinline__ void arrive(uint32_t addr, bool remote) {
+    if (remote)
+        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    else
+        asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 
 // What an Op needs to know of where it runs.
@@ -297,6 +314,9 @@ struct Ctx {
 };
 
 // The kernel body. Op (a __grid_constant__ parameter) has
+//   SWAP                   compile-time, CG 1: not 0 where the second operand's rows lie along TMEM's
+//                          lanes (128 at a time, two runs to an accumulator) and SWAP rows of the first
+//                          along its columns: for few rows, whose 128 would be mostly padding
 //   CG, F8, PROMOTE, EPI   compile-time: CTAs per tile, 8-bit operands, join accumulators in registers,
 //                          epilogue warps
 //   format                 operand format of the instruction descriptor
@@ -352,7 +372,8 @@ __device__ __forceinline__ void run(const Op& op) {
     ctx.kept = op.kept();
 
     Tile t;
-    const uint32_t acc_cols = op.n <= 64 ? 64 : op.n <= 128 ? 128 : 256, accs = 512 / acc_cols;
+    const uint32_t acc_cols = Op::SWAP ? 2 * Op::SWAP : op.n <= 64 ? 64 : op.n <= 128 ? 128 : 256;
+    const uint32_t accs = min(512 / acc_cols, (uint32_t)MAX_ACC);
     if (warp < EPI_WARP0) {
         if constexpr (Op::EPI == 16)
             asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -394,7 +415,7 @@ __device__ __forceinline__ void run(const Op& op) {
             bool ok = true;
             for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
                 const bool amn = op.a_mn(t), bmn = op.b_mn(t);
-                const uint32_t idesc = instr_desc(op.format, amn, bmn, 128 * CG, t.n);
+                const uint32_t idesc = instr_desc(op.format, amn, bmn, 128 * CG, Op::SWAP ? Op::SWAP : t.n);
                 // K-major: 8-row groups 1024 bytes apart, a step of K is 32 bytes of the row.
                 // MN-major: 64-wide slabs of 64 k rows (8192 bytes), 8-k groups 1024 bytes
                 // apart, a step of 16 k rows is 2048 bytes.
@@ -413,9 +434,17 @@ __device__ __forceinline__ void run(const Op& op) {
                     if (elect()) {
                         const uint64_t da = da0 + (uint64_t)(s * (G::STAGE >> 4)), db = db0 + (uint64_t)(s * (G::STAGE >> 4));
                         const uint32_t d = tmem + buf * acc_cols;
+                        if (Op::SWAP) {
+                            for (int h = 0; h * 128 < t.n; ++h)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<CG, Op::F8>(d, da + k * step_a, db + k * step_b, idesc, k > 0 || in > 0);
+                                for (int k = 0; k < 4; ++k)
+                                    mma<CG, Op::F8>(d + h * Op::SWAP, db + h * (128 * ROW >> 4) + k * step_b,
+                                                    da + k * step_a, idesc, k > 0 || in > 0);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma<CG, Op::F8>(d, da + k * step_a, db + k * step_b, idesc, k > 0 || in > 0);
+                        }
                         commit<CG>(&ring->empty[s]);
                         if (last) commit<CG>(&ring->tfull[buf]);
                     }
@@ -446,7 +475,8 @@ __device__ __forceinline__ void run(const Op& op) {
         me.row = (int)ctx.rank * 128 + me.quad * 32 + lane;
         me.xpose = xpose + (warp - EPI_WARP0) * G::XPOSE;
         const uint32_t lanes = (uint32_t)(me.quad * 32) << 16;
-        const uint32_t te0 = CG == 2 ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
+        const bool remote = CG == 2 && ctx.rank != 0;
+        const uint32_t te0 = remote ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
         uint32_t buf = 0, tph = 0;
         bool ok = true;
         for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
@@ -467,7 +497,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     op.join(acc, t, tmem + buf * acc_cols + lanes, me, ctx, [&] {
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) arrive_remote(te0 + buf * 8);
+                        if (lane == 0) arrive(te0 + buf * 8, remote);
                     });
                     if (++buf == accs) buf = 0, tph ^= 1;
                 }
@@ -479,7 +509,7 @@ __device__ __forceinline__ void run(const Op& op) {
                 op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx);
                 fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_remote(te0 + buf * 8);
+                if (lane == 0) arrive(te0 + buf * 8, remote);
                 if (++buf == accs) buf = 0, tph ^= 1;
             }
         }
