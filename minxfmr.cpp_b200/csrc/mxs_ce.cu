@@ -351,50 +351,54 @@ __device__ __forceinline__ void join_pair(float& m, float& s, float om, float os
     m = nm;
 }
 
-// Joins the tiles' pairs of a row, in the same order every time: a warp per row,
-// or (whole: few rows, where a warp's chain of reads would be most of the call)
-// a CTA.
+// Joins the tiles' pairs of a row, in the same order every time. Few rows (WHOLE): a
+// CTA a row. Many: a CTA for 32 rows, a lane each, so that the pairs of neighbouring
+// rows are read together, its 8 warps an eighth of the tiles each.
+template <bool WHOLE>
 __global__ void __launch_bounds__(256) score_join_kernel(const float2* part, const float* ytarget, const int* pos,
-                                                         Targets targets, int rows, int tiles, bool whole,
-                                                         float* loss, float* lse) {
-    __shared__ float2 s_pair[8];
+                                                         Targets targets, int rows, int tiles, float* loss,
+                                                         float* lse) {
+    __shared__ float2 s_pair[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = whole ? blockIdx.x : blockIdx.x * 8 + warp;
+    const int r = WHOLE ? blockIdx.x : blockIdx.x * 32 + lane;
     mxs::gemm::grid_wait();
     mxs::gemm::grid_launch_dependents();
-    if (r >= rows) return;
-    int at = targets(r) >= 0 ? r : -1;
-    if (pos) at = pos[r];
-    if (at < 0) {
-        if (whole ? threadIdx.x == 0 : lane == 0) {
-            if (loss) loss[r] = 0.0f;
-            if (lse) lse[r] = 0.0f;
-        }
-        return;
+    int at = -1;
+    if (r < rows) {
+        at = targets(r) >= 0 ? r : -1;
+        if (pos) at = pos[r];
     }
     float m = -INFINITY, s = 0.0f;
-    const int step = whole ? 256 : 32;
-#pragma unroll 4
-    for (int i = whole ? threadIdx.x : lane; i < tiles; i += step) {
-        const float2 q = part[(int64_t)i * rows + at];
+    if (at >= 0) {
+        const int per = (tiles + 7) / 8;
+        const int from = WHOLE ? threadIdx.x : warp * per, to = WHOLE ? tiles : min(tiles, from + per);
+#pragma unroll 8
+        for (int i = from; i < to; i += WHOLE ? 256 : 1) {
+            const float2 q = part[(int64_t)i * rows + at];
+            join_pair(m, s, q.x, q.y);
+        }
+    }
+    if (WHOLE) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            join_pair(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    }
+    if (!WHOLE || lane == 0) s_pair[warp][WHOLE ? 0 : lane] = make_float2(m, s);
+    __syncthreads();
+    if (WHOLE ? threadIdx.x != 0 : warp != 0 || r >= rows) return;
+    for (int w = 1; w < 8; ++w) {
+        const float2 q = s_pair[w][WHOLE ? 0 : lane];
         join_pair(m, s, q.x, q.y);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-        join_pair(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
-    if (whole) {
-        if (lane == 0) s_pair[warp] = make_float2(m, s);
-        __syncthreads();
-        if (threadIdx.x != 0) return;
-        for (int w = 1; w < 8; ++w) join_pair(m, s, s_pair[w].x, s_pair[w].y);
-    }
-    if (lane == 0) {
+    float l = 0.0f, e = 0.0f;  // a row left out
+    if (at >= 0) {
         const float y = ytarget[at];
         const float diff = (m + log2f(s) - y) * LN2;  // others' log-sum minus the target's logit
-        const float l = fmaxf(diff, 0.0f) + log1pf(expf(-fabsf(diff)));
-        if (loss) loss[r] = l;
-        if (lse) lse[r] = fmaf(y, LN2, l);
+        l = fmaxf(diff, 0.0f) + log1pf(expf(-fabsf(diff)));
+        e = fmaf(y, LN2, l);
     }
+    if (loss) loss[r] = l;
+    if (lse) lse[r] = e;
 }
 
 // The logits of a piece again, left as G = ghat (softmax - hot) in the operands'
@@ -591,9 +595,12 @@ __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, 
 // ---------------------------------------------------------------------------
 // Plan
 // ---------------------------------------------------------------------------
-// G is held for a piece of the vocabulary at a time: about this many bytes, so
-// that the two products that read it find it in L2.
-constexpr int64_t PIECE_BYTES = 64 << 20;
+// G is held for a piece of the vocabulary at a time, of about this many bytes. A
+// piece costs two launches whose last tiles leave pairs idle, so larger ones are
+// faster, with less and less to gain; L2 holds none of them beside its operands.
+// Loss and gradients of 4096 x 151936 x 3584: 13.57 ms with 64 MB, 13.2 with 128,
+// 13.0 with 512.
+constexpr int64_t PIECE_BYTES = 256 << 20;
 
 struct Plan {
     Head* head;
@@ -741,10 +748,13 @@ int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss
     op.ytarget = pl.ytarget;
     const int64_t units = CG == 1 ? ceil_div(a.vocab, pl.span) : ceil_div(a.rows, 256) * pl.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
-    const bool whole = a.rows <= a.sms * 2;
-    MXS_TRY(launch_dependent(score_join_kernel, (unsigned)(whole ? a.rows : ceil_div(a.rows, 8)), 256, a.st, pl.part,
-                             pl.ytarget, pl.direct ? nullptr : pl.pos, a.targets, (int)a.rows, pl.nt, whole, loss,
-                             lse));
+    const int* pos = pl.direct ? nullptr : pl.pos;
+    if (a.rows <= 64)
+        MXS_TRY(launch_dependent(score_join_kernel<true>, (unsigned)a.rows, 256, a.st, pl.part, pl.ytarget, pos,
+                                 a.targets, (int)a.rows, pl.nt, loss, lse));
+    else
+        MXS_TRY(launch_dependent(score_join_kernel<false>, (unsigned)ceil_div(a.rows, 32), 256, a.st, pl.part,
+                                 pl.ytarget, pos, a.targets, (int)a.rows, pl.nt, loss, lse));
     return MXS_OK;
 }
 

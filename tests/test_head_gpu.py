@@ -416,3 +416,101 @@ def test_refusals(mxs):
     rc = lib.mxs_ce_from_hidden(P(h.data_ptr()), 16, P(w.data_ptr()), 16, 0, 4, 16, 20, P(t.data_ptr()), 8, 1.0,
                                 P(loss.data_ptr()), None, P(ws.data_ptr()), 64, None)
     assert rc == mxs.MXS_ERR_WORKSPACE
+
+
+# ---------------------------------------------------------------------------
+# Large offsets, give-ups, the example
+# ---------------------------------------------------------------------------
+
+def test_offsets_past_32_bits(mxs):
+    """A weight of 2.24e9 elements: the last vocabulary rows' logits, targets and
+    gradients, against the formula on those rows (lse from pieces in doubles)."""
+    rows, vocab, d = 3, 140000, 16000
+    g = gen(31)
+    w = torch.empty((vocab, d), dtype=BF, device="cuda")
+    for i in range(0, vocab, 10000):
+        w[i:i + 10000] = torch.randn((10000, d), generator=g, device="cuda") * (2.5 / math.sqrt(d))
+    h = torch.randn((rows, d), generator=g, device="cuda").to(BF)
+    t = torch.tensor([vocab - 1, 5, vocab - 700], device="cuda")
+    loss, lse = mxs.ce_from_hidden(h, w, t)
+    x = torch.cat([h.double() @ w[i:i + 10000].double().t() for i in range(0, vocab, 10000)], 1)
+    tol = head_ref.logit_tol(h, w[:10000], 1.0)  # rows of one distribution: the largest norm of 10000 stands for all
+    want = torch.logsumexp(x, 1)
+    assert ((lse.double() - want).abs() <= 2 * tol + 1e-5).all()
+    assert ((loss.double() - (want - x.gather(1, t[:, None])[:, 0])).abs() <= 4 * tol + 1e-5).all()
+    grad = torch.tensor([1.0, -0.5, 2.0], device="cuda")
+    _, gw = mxs.ce_from_hidden_backward(h, w, t, lse, grad, need_hidden=False)
+    p = torch.exp(x - want[:, None])
+    p.scatter_add_(1, t[:, None], torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
+    p *= grad.double()[:, None]
+    for part in (slice(0, 300), slice(vocab - 1000, vocab)):
+        dw = p[:, part].t() @ h.double()
+        mag = p[:, part].abs().t() @ h.double().abs()
+        # G and the result rounded to bf16 (2^-8 each), the probabilities' own error
+        assert ((gw[part].double() - dw).abs() <= (2 * 2.0 ** -8 + 4 * tol) * mag + 1e-30).all()
+
+
+def test_output_offsets_past_32_bits(mxs):
+    """An 8-bit product with 2.4e9 outputs: its last rows against those computed alone."""
+    a, sa, b, sb = fp8_operands(16000, 300, 128, seed=3)
+    b, sb = b.view(torch.uint8).repeat(500, 1).view(torch.float8_e4m3fn), None
+    n = b.shape[0]  # 150000
+    sb = torch.rand((-(-n // 128), 1), generator=gen(5), device="cuda") + 0.5
+    out = mxs.matmul_fp8(a, sa, b, sb, out_dtype=BF)
+    check = mxs.matmul_fp8(a[15990:], sa[15990:], b, sb, out_dtype=BF)
+    assert torch.equal(out[15990:], check)
+    want, tol = head_ref.matmul_fp8(a[15990:], sa[15990:], b, sb, BF)
+    assert ((check.double() - want).abs() <= tol).all()
+
+
+def big_head(mxs):
+    h, w, t = operands(300, 20000, 512, BF, seed=40)
+    a = fp8_operands(300, 9000, 512)
+    few = (a[0][:20], a[1][:20], a[2], a[3])
+    mid = (a[0][:100], a[1][:100], a[2], a[3])
+    loss, lse = mxs.ce_from_hidden(h, w, t)
+    grad = torch.ones(300, device="cuda")
+    return {
+        "loss": lambda: mxs.ce_from_hidden(h, w, t),
+        "loss of few rows": lambda: mxs.ce_from_hidden(h[:9], w, t[:9]),
+        "gradients": lambda: mxs.ce_from_hidden_backward(h, w, t, lse, grad),
+        "product": lambda: (mxs.matmul_fp8(*a),),
+        "product of some rows": lambda: (mxs.matmul_fp8(*mid),),
+        "product of few rows": lambda: (mxs.matmul_fp8(*few),),
+    }
+
+
+@pytest.mark.parametrize("name", ["loss", "loss of few rows", "gradients", "product", "product of some rows",
+                                  "product of few rows"])
+def test_bounded_waits_give_up(mxs, name):
+    """A producer that stops before one of its copies (a test hook): the waits give
+    up after about a second, the status word says so, nothing hangs, and the next
+    call on the same inputs gives the same bits as before."""
+    call = big_head(mxs)[name]
+    before = call()
+    torch.cuda.synchronize()
+    mxs.get_status(clear=True)
+    mxs.set_test_hooks(drop_tile=1)  # every case has two blocks for its first CTA
+    try:
+        call()
+        torch.cuda.synchronize()
+    finally:
+        mxs.set_test_hooks()
+    assert mxs.get_status(clear=True) & mxs.ROW_TIMEOUT
+    after = call()
+    torch.cuda.synchronize()
+    assert mxs.get_status(clear=True) == 0
+    for x, y in zip(before, after):
+        assert torch.equal(x, y)
+
+
+def test_example_learns(mxs):
+    """The example's step (8-bit draw, score, gradient, update): the reward rises."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import head_step
+    log = head_step.train(rows=128, d=256, vocab=4000, steps=25)
+    first, last = sum(r for r, _ in log[:5]) / 5, sum(r for r, _ in log[-5:]) / 5
+    assert all(math.isfinite(l) for _, l in log)
+    assert last > first
