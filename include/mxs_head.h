@@ -47,7 +47,7 @@ extern "C" {
  *             is not read (it may hold NaN), and it costs no products.
  *   d_loss, d_lse  rows floats; either may be NULL
  * Products are exact in fp32 and accumulated in fp32; maxima and sums of the
- * softmax are fp32. Limits: vocab, rows, d_model < 2^31; temperature > 0.
+ * softmax are fp32. Limits: vocab, rows, d_model < 2^31 - 1024; temperature > 0.
  */
 MXS_API int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
                                int dtype, int64_t rows, int64_t d_model, int64_t vocab, const void* d_targets,
@@ -62,8 +62,10 @@ MXS_API int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const vo
  *   grad_weight_v = 1 / temperature * sum_r grad_loss_r P[r][v] hidden_r
  * Both are written whole (rows left out get a zero gradient); either may be NULL
  * and is then not computed. The logits are computed again, a piece of the
- * vocabulary at a time; a piece of P is held in `dtype`, sums are fp32, and the
- * gradients are rounded to `dtype` once.
+ * vocabulary at a time; a piece of grad_loss_r P[r][v] / max |grad_loss| is held in
+ * `dtype` (for MXS_F16 entries below 2^-28 of the largest weight lose precision),
+ * what that rounding leaves out of a row's target entry is kept in fp32, sums are
+ * fp32, and the gradients are rounded to `dtype` once.
  */
 MXS_API int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const void* d_weight,
                                         int64_t ld_weight, int dtype, int64_t rows, int64_t d_model, int64_t vocab,
@@ -100,7 +102,7 @@ MXS_API int mxs_quantize_fp8(const void* d_x, int64_t ld_x, int dtype, int64_t r
  * for each 1 x 128 block of a and each 128 x 128 block of b, as
  * mxs_quantize_fp8 makes them. Each block of 128 products is summed in fp32 and
  * joined under its scales in fp32; out (MXS_F32, MXS_BF16 or MXS_F16; leading
- * dimension ld_out) is rounded once. Limits: rows, n, k < 2^31.
+ * dimension ld_out) is rounded once. Limits: rows, n, k < 2^31 - 1024.
  */
 MXS_API int mxs_matmul_fp8(const void* d_a, int64_t ld_a, const float* d_a_scale, const void* d_b, int64_t ld_b,
                            const float* d_b_scale, int64_t rows, int64_t n, int64_t k, void* d_out, int64_t ld_out,

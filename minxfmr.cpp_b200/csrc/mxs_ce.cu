@@ -13,12 +13,17 @@
 //   G[r][v] = ghat_r (2^(y_v - lse_r log2 e) - (v == t_r)),   ghat = grad / max |grad|,
 // held in the operands' type, then grad_hidden += G W and grad_weight = G^T H,
 // each times max|grad| / temperature once, in fp32, at the end. Dividing by
-// max |grad| keeps a batch mean's 1/rows out of G: the target's entry is then
-// near -1, which both types hold with no error common to a whole row.
+// max |grad| keeps a batch mean's 1/rows out of G and its range in the types';
+// what the rounding of a row's target entry, its largest, leaves out is added to
+// both gradients in fp32.
 //
 // Rows whose target is out of range are packed away first (pack_rows_kernel), so
 // they cost no products; every later kernel reads the number of rows left from
-// device memory.
+// device memory. (Forward, up to 128 aligned rows: read in place instead.)
+//
+// Bound by the tensor cores from some hundred rows on (512 clocks of MMA for each
+// 64 of K and 256 x 256 tile; at 4096 x 151936 x 3584 the power limit holds the
+// clock near 1.4 GHz), by the weight's bytes below.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -298,12 +303,12 @@ struct LogitTiles {
 // clocks of MMA for each 64 of d_model.
 // The MMA's own fp32 sum rounds towards zero at every 16 products, which at
 // d_model 3584 leaves 2e-6 of the logits' size; joining the accumulator in
-// registers (round to nearest) every 1024 products keeps it below 1e-6 and costs
-// one more read of the accumulator for each.
+// registers (round to nearest) every 512 products keeps it near 5e-7, as a plain
+// fp32 product has it, and costs one more read of the accumulator for each.
 template <int CG_>
 struct ScoreOp : LogitTiles<CG_> {
     static constexpr bool PROMOTE = true;
-    __device__ int group() const { return 16; }
+    __device__ int group() const { return 8; }
     struct Acc {
         float v[2][32];
     };

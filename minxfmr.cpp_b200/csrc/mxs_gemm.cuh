@@ -100,7 +100,9 @@ __device__ __forceinline__ bool elect() {
     return p != 0;
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 // 2-D tile load; `bar` is a shared::cluster address (with CG = 2, the even CTA's barrier).
 template <int CG>
@@ -121,9 +123,11 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
     if (CG == 2)
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot))
+                     : "memory");
     else
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot))
+                     : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tmem_free(uint32_t base) {
@@ -432,7 +436,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     fence_after();
                     const bool last = in + 1 == group || kb == t.kn - 1;
                     if (elect()) {
-                        const uint64_t da = da0 + (uint64_t)(s * (G::STAGE >> 4)), db = db0 + (uint64_t)(s * (G::STAGE >> 4));
+                        const uint64_t at = s * (G::STAGE >> 4), da = da0 + at, db = db0 + at;
                         const uint32_t d = tmem + buf * acc_cols;
                         if (Op::SWAP) {
                             for (int h = 0; h * 128 < t.n; ++h)
