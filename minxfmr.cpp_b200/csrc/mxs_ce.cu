@@ -52,14 +52,25 @@ struct Head {
     float gmax;    // largest finite |grad_loss| of those rows (1 if none)
 };
 
-// Splits of K for `tiles` grad_hidden tiles: as many as fill the units, at least
-// 8 blocks of 64 columns each. A fixed function of the shape: the same sums in the same order every time.
-__host__ __device__ inline int grad_hidden_splits(int tiles, int width, int units) {
-    const int blocks = (width + 63) / 64, most = (blocks + 7) / 8;
-    int s = tiles > 0 ? units / tiles : 1;
-    s = s < 1 ? 1 : s < most ? s : most;
-    const int per = (blocks + s - 1) / s;
-    return (blocks + per - 1) / per;  // none of them empty
+// Splits of K for the grad_hidden tiles of a piece of `width` columns: so many that
+// one split takes about a unit's share of the launch's work, grad_weight's tiles
+// included (a tile of few blocks counts as 8: its epilogue takes as long as those),
+// at least 8 blocks of 64 columns each, and no more than fill the units. A fixed
+// function of the shape: the same sums in the same order every time.
+// (One split per unit, 36 of them, instead of these 13 in a step of 200 x 32000 x 512 cost @@A@@.)
+__host__ __device__ inline int grad_hidden_splits(int kept, int nt, int width, int units, bool want_w) {
+    const int64_t tiles = (int64_t)((kept + 255) / 256) * nt;
+    if (tiles == 0) return 1;
+    const int64_t blocks = (width + 63) / 64, rows = (kept + 63) / 64;
+    const int64_t other = want_w ? (int64_t)((width + 255) / 256) * nt * (rows > 8 ? rows : 8) : 0;
+    const int64_t work = tiles * blocks + other;
+    int64_t s = (blocks * units + work - 1) / work;
+    const int64_t most = (blocks + 7) / 8, fill = units / tiles;
+    s = s < most ? s : most;
+    s = s < fill ? s : fill;
+    s = s < 1 ? 1 : s;
+    const int64_t per = (blocks + s - 1) / s;
+    return (int)((blocks + per - 1) / per);  // none of them empty
 }
 
 // The caller's targets: the row's, or -1 where it is outside the vocabulary.
@@ -532,7 +543,7 @@ struct ProductOp {
     // with one tile fewer, those take the grad_weight tiles of the same cost before the rest go round.
     __device__ bool tile(int i, const Ctx& x, Tile& t) const {
         const int mh = want_h ? (x.kept + 255) / 256 : 0, th = mh * nt;
-        const int splits = grad_hidden_splits(th, split_width, x.units);
+        const int splits = grad_hidden_splits(want_h ? x.kept : 0, nt, split_width, x.units, want_w);
         const int kh = (width + 63) / 64, kw = (x.kept + 63) / 64;
         const int nh = th * splits;
         const int mine = (nh - x.unit + x.units - 1) / x.units;  // grad_hidden tiles of this unit
@@ -547,7 +558,8 @@ struct ProductOp {
         if (!want_w) return false;
         const int64_t total = (int64_t)((width + 255) / 256) * nt;
         const int over = nh % x.units;  // units [0, over) have one tile more
-        const int ahead = over == 0 || kw == 0 ? 0 : ((kh + splits - 1) / splits + kw / 2) / kw;
+        const int cost = max(kw, 8);  // of a grad_weight tile, in blocks
+        const int ahead = over == 0 ? 0 : ((kh + splits - 1) / splits + cost / 2) / cost;
         int j = i - mine;
         int64_t idx;
         if (x.unit >= over && j < ahead) {
@@ -643,7 +655,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, const int* pos, const Head* head,
                                                               const int* target, const Link* link, const T* w,
                                                               int64_t ldw, int d, int n, int width, int units,
-                                                              float scale, T* out, int64_t ld) {
+                                                              bool want_w, float scale, T* out, int64_t ld) {
     mxs::gemm::grid_wait();
     mxs::gemm::grid_launch_dependents();
     const int64_t r = blockIdx.y;
@@ -652,7 +664,7 @@ __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, 
     const int at = pos[r];
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (at >= 0) {
-        const int nt = (d + n - 1) / n, splits = grad_hidden_splits((head->kept + 255) / 256 * nt, width, units);
+        const int nt = (d + n - 1) / n, splits = grad_hidden_splits(head->kept, nt, width, units, want_w);
         const int64_t tile = (int64_t)(at / 256) * nt + k / n;
         const float* a = acc + (tile * splits * 256 + at % 256) * 256 + k % n;
 #pragma unroll 8
@@ -942,7 +954,7 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
         const dim3 grid((unsigned)ceil_div(a.d, 512), (unsigned)std::min<int64_t>(65535, a.rows - r));
         MXS_TRY(launch_dependent(grad_hidden_out_kernel<T>, grid, 128, a.st, pl.acc, pl.pos + r, pl.head, pl.target,
                                  pl.link, static_cast<const T*>(w), ldw, (int)a.d, pl.dn, prod.split_width, a.sms / 2,
-                                 prod.scale, static_cast<T*>(gh) + r * ldgh, ldgh));
+                                 prod.want_w, prod.scale, static_cast<T*>(gh) + r * ldgh, ldgh));
     }
     return MXS_OK;
 }
