@@ -458,7 +458,8 @@ struct DecodeOp {
 
 template <int CG, typename O, int RUNS>
 int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
-                 int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status, cudaStream_t st) {
+                 int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status,
+                 cudaStream_t st) {
     MatmulOp<CG, O, RUNS> op{};
     op.format = 0;
     op.drop = mxs::test_drop_tile();
@@ -481,8 +482,8 @@ int launch_tiles(const void* a, int64_t lda, const float* sa, const void* b, int
 }
 
 template <typename O, int NP>
-int launch_decode(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
-                  int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status,
+int launch_decode(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb,
+                  int64_t rows, int64_t n, int64_t k, void* out, int64_t ldo, int width, int span, int sms, uint32_t* status,
                   cudaStream_t st) {
     DecodeOp<O, NP> op{};
     op.format = 0;
@@ -495,14 +496,15 @@ int launch_decode(const void* a, int64_t lda, const float* sa, const void* b, in
     op.a_rows = (int)round_up(rows, 8);  // rows that the box leaves out give columns nobody reads
     op.out = static_cast<O*>(out);
     op.ldo = ldo;
-    if (!mxs::gemm::make_map(&op.ma, a, 1, k, rows, lda, op.a_rows) || !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, 32))
+    if (!mxs::gemm::make_map(&op.ma, a, 1, k, rows, lda, op.a_rows) ||
+        !mxs::gemm::make_map(&op.mb, b, 1, k, n, ldb, 32))
         return MXS_ERR_CUDA;
     return mxs::gemm::launch(op, (int)ceil_div(n, span), st) == cudaSuccess ? MXS_OK : MXS_ERR_CUDA;
 }
 
 template <typename O>
-int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t rows,
-                  int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
+int launch_matmul(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb,
+                  int64_t rows, int64_t n, int64_t k, void* out, int64_t ldo, int sms, uint32_t* status, cudaStream_t st) {
     const int span = (int)round_up(ceil_div(n, sms), 32);  // up to 128 rows: one tile of them
     const int w = rows > 128 ? mxs::tile_width(ceil_div(rows, 256), n, sms / 2, 64, 32)
                              : (int)round_up(ceil_div(span, ceil_div(span, 256)), 32);
