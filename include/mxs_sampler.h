@@ -306,6 +306,8 @@ MXS_API int mxs_sample_topk_noalloc(const float* d_logits, int64_t rows, int64_t
  *   drop_tile        CTA 0's streaming producer stops before its tile with this
  *                    sequence number, so its consumers' bounded wait runs out and
  *                    the rows report MXS_ROW_TIMEOUT (-1: off, the default)
+ *                    (calls of mxs_head.h: CTA 0's operand producer stops before this
+ *                    block of operands, and the status word reports it)
  *   replay_warp_min  a finish CTA replays its tie rows one per warp when it holds
  *                    at least this many, else with the whole CTA (default 1)
  *   path             0: default planning; 2: the CTA-synchronous kernel for every k
