@@ -150,14 +150,32 @@ class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_loss):
         hidden, weight, targets, lse = ctx.saved_tensors
-        gh, gw = ce_from_hidden_backward(hidden, weight, targets, lse, grad_loss.float().contiguous(),
-                                         ctx.temperature, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        with torch.no_grad():
+            gh, gw = ce_from_hidden_backward(hidden, weight, targets, lse, grad_loss.float().contiguous(),
+                                             ctx.temperature, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        if torch.is_grad_enabled():  # create_graph
+            gh, gw = _DifferentiatedOnce.apply(gh, gw, hidden, weight, grad_loss)
         return gh, gw, None, None
 
 
+class _DifferentiatedOnce(torch.autograd.Function):
+    """Gradients with a place in the graph of what they were computed from, where
+    differentiating them raises. (torch's once_differentiable looks at grad_loss
+    alone: a constant one, a plain sum's, would leave the gradients without a graph
+    and a second derivative without their part.)"""
+
+    @staticmethod
+    def forward(ctx, gh, gw, hidden, weight, grad_loss):
+        return gh, gw
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("cross_entropy_from_hidden can be differentiated once only")
+
+
 def cross_entropy_from_hidden(hidden, weight, targets, temperature=1.0):
-    """ce_from_hidden's loss [rows] as a differentiable function of hidden and
-    weight, for torch.autograd."""
+    """ce_from_hidden's loss [rows] as a function of hidden and weight that
+    torch.autograd can differentiate once (second derivatives raise)."""
     return _CrossEntropy.apply(hidden, weight, targets, float(temperature))
 
 
