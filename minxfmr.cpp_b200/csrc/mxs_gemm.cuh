@@ -408,12 +408,18 @@ __device__ __forceinline__ void run(const Op& op) {
                     if (++s == G::STAGES) s = 0, ph ^= 1;
                 }
             }
-            // gave up: the copies still in flight (at most one per stage) land before the CTA ends
-            if (!ok && ctx.rank == 0) {
-                const int64_t n = issued < G::STAGES ? issued : (int64_t)G::STAGES;
-                for (int64_t j = issued - n; j < issued; ++j)
+            // What the last blocks (at most one per stage) still send to this CTA's barriers lands
+            // before the CTA ends: the MMAs' hand-backs of their stages, which the pair's even CTA
+            // sends to both, or, after a give-up, the copies and the even CTA's word that its MMAs
+            // have finished.
+            const int64_t last = issued < G::STAGES ? issued : (int64_t)G::STAGES;
+            for (int64_t j = issued - last; ok && j < issued; ++j)
+                ok = __all_sync(0xffffffffu, wait(&ring->empty[j % G::STAGES], (uint32_t)(j / G::STAGES) & 1, ring));
+            if (!ok && ctx.rank == 0)
+                for (int64_t j = issued - last; j < issued; ++j)
                     mbar_wait_bounded(&ring->full[j % G::STAGES], (uint32_t)(j / G::STAGES) & 1);
-            }
+            else if (!ok)
+                mbar_wait_bounded(&ring->drain, 0);
         } else if (warp == 1 && ctx.rank == 0) {
             uint32_t s = 0, ph = 0, buf = 0, tph = 0;
             bool ok = true;
