@@ -347,7 +347,7 @@ struct ScoreOp : LogitTiles<CG_> {
         }
         release();
     }
-    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx& x) const {
+    __device__ void finish(Acc& a, const Tile& t, Lane& me, const Ctx& x) const {
         const int r = t.m0 + me.row;
         if ((r & ~31) >= x.kept) return;  // the four warps of these rows agree
         const int hit = r < x.kept ? this->target_of(r) - t.n0 : -1;  // the target's column of this tile
@@ -382,8 +382,10 @@ struct ScoreOp : LogitTiles<CG_> {
             s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
             m = nm;
         }
-        // two buffers: a warp is at most one tile ahead of the others of its rows
-        float2* mine = reinterpret_cast<float2*>(me.xpose) + (t.seq & 1) * 32 + me.lane;
+        // Two buffers, taken in turn by the meetings (not by the tiles, some of which these warps
+        // skip): what is written for one meeting is read before that warp comes to the next, and
+        // overwritten only after it.
+        float2* mine = reinterpret_cast<float2*>(me.xpose) + (me.meetings++ & 1) * 32 + me.lane;
         *mine = make_float2(m, s);
         asm volatile("bar.sync %0, 128;" ::"r"(me.quad + 1) : "memory");
         if (me.grp != 0 || r >= x.kept) return;

@@ -62,7 +62,6 @@ struct Tile {
     int k0, kn;   // first k block and number of blocks
     int n;        // columns of the MMA
     int kind;     // Op's own
-    int seq;      // which of this unit's tiles
 };
 
 // An epilogue thread's place.
@@ -70,6 +69,7 @@ struct Lane {
     int lane, quad, grp;  // quad: which 32 rows of the CTA's 128; grp: which column group
     int row;              // of the pair's tile
     uint8_t* xpose;       // its warp's bytes for transposes
+    int meetings;         // Op's own, 0 at the start: how often the warps of this quad have met
 };
 
 struct Ring {
@@ -484,13 +484,13 @@ __device__ __forceinline__ void run(const Op& op) {
         me.grp = (warp - EPI_WARP0) >> 2;
         me.row = (int)ctx.rank * 128 + me.quad * 32 + lane;
         me.xpose = xpose + (warp - EPI_WARP0) * G::XPOSE;
+        me.meetings = 0;
         const uint32_t lanes = (uint32_t)(me.quad * 32) << 16;
         const bool remote = CG == 2 && ctx.rank != 0;
         const uint32_t te0 = remote ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
         uint32_t buf = 0, tph = 0;
         bool ok = true;
         for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
-            t.seq = i;
             if (t.kn == 0) {  // an empty sum: no product, no accumulator
                 op.zero(t, me, ctx);
                 continue;
