@@ -307,7 +307,8 @@ MXS_API int mxs_sample_topk_noalloc(const float* d_logits, int64_t rows, int64_t
  *                    sequence number, so its consumers' bounded wait runs out and
  *                    the rows report MXS_ROW_TIMEOUT (-1: off, the default)
  *                    (calls of mxs_head.h: CTA 0's operand producer stops before this
- *                    block of operands, and the status word reports it)
+ *                    block of operands, and the status word reports it; below -1, CTA 0's
+ *                    first epilogue warp leaves before its tile -2 - drop_tile)
  *   replay_warp_min  a finish CTA replays its tie rows one per warp when it holds
  *                    at least this many, else with the whole CTA (default 1)
  *   path             0: default planning; 2: the CTA-synchronous kernel for every k

@@ -347,9 +347,9 @@ struct ScoreOp : LogitTiles<CG_> {
         }
         release();
     }
-    __device__ void finish(Acc& a, const Tile& t, Lane& me, const Ctx& x) const {
+    __device__ bool finish(Acc& a, const Tile& t, Lane& me, const Ctx& x) const {
         const int r = t.m0 + me.row;
-        if ((r & ~31) >= x.kept) return;  // the four warps of these rows agree
+        if ((r & ~31) >= x.kept) return true;  // the four warps of these rows agree
         const int hit = r < x.kept ? this->target_of(r) - t.n0 : -1;  // the target's column of this tile
         const int cols = min(t.n, this->vocab - t.n0);
         float m = -INFINITY, s = 0.0f;
@@ -385,10 +385,10 @@ struct ScoreOp : LogitTiles<CG_> {
         // Two buffers, taken in turn by the meetings (not by the tiles, some of which these warps
         // skip): what is written for one meeting is read before that warp comes to the next, and
         // overwritten only after it.
-        float2* mine = reinterpret_cast<float2*>(me.xpose) + (me.meetings++ & 1) * 32 + me.lane;
+        float2* mine = reinterpret_cast<float2*>(me.xpose) + (me.meetings & 1) * 32 + me.lane;
         *mine = make_float2(m, s);
-        asm volatile("bar.sync %0, 128;" ::"r"(me.quad + 1) : "memory");
-        if (me.grp != 0 || r >= x.kept) return;
+        if (!mxs::gemm::meet(me, x)) return false;
+        if (me.grp != 0 || r >= x.kept) return true;
 #pragma unroll
         for (int g = 1; g < 4; ++g) {  // group g's warp is four places on
             const float2 q = mine[g * 4 * (mxs::gemm::XPOSE_ALL / LogitTiles<CG_>::EPI / 8)];
@@ -397,6 +397,7 @@ struct ScoreOp : LogitTiles<CG_> {
             m = nm;
         }
         part[(int64_t)t.kind * this->rows + r] = make_float2(m, s);
+        return true;
     }
 };
 

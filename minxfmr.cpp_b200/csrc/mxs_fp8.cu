@@ -350,9 +350,9 @@ struct MatmulOp {
             for (int j = 0; j < 32; ++j) a.v[i][j] = fmaf(x[j], a.now[i], a.v[i][j]);
         }
     }
-    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
+    __device__ bool finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
         const int r0 = t.m0 + me.row - me.lane;
-        if (r0 >= rows) return;
+        if (r0 >= rows) return true;
         O* o = out + (int64_t)r0 * ldo + t.n0;
 #pragma unroll
         for (int i = 0; i < RUNS; ++i) {
@@ -360,6 +360,7 @@ struct MatmulOp {
             if (c0 >= t.n) break;
             mxs::gemm::store_rows<O, false, 32 * sizeof(O)>(o + c0, ldo, a.v[i], rows - r0, cols - t.n0 - c0, vec, me);
         }
+        return true;
     }
 };
 
@@ -446,13 +447,14 @@ struct DecodeOp {
             }
         }
     }
-    __device__ void finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
+    __device__ bool finish(Acc& a, const Tile& t, const Lane& me, const Ctx&) const {
         const int c = first(me) + me.lane;
-        if (c >= t.n || t.n0 + c >= cols) return;
+        if (c >= t.n || t.n0 + c >= cols) return true;
         O* o = out + t.n0 + c;
 #pragma unroll
         for (int i = 0; i < NP; ++i)
             if (i < rows) o[(int64_t)i * ldo] = mxs::from_f32<O>(a.v[i]);
+        return true;
     }
 };
 

@@ -26,8 +26,8 @@
 // so all three products of a loss and its gradients read the same row-major
 // matrices without a transposed copy.
 //
-// Every wait is bounded (about 1 s, as in the streaming kernel); a wait that
-// gives up marks the CTA dead, its roles stop, copies and MMAs in flight are
+// Every wait is bounded (about 1 s, as in the streaming kernel), the epilogue warps'
+// for one another too; a wait that gives up marks the CTA dead, its roles stop, copies and MMAs in flight are
 // waited for (bounded again), TMEM is freed, and the device's status word gets
 // FLAG_TIMEOUT. No TMA multicast anywhere.
 #pragma once
@@ -69,11 +69,12 @@ struct Lane {
     int lane, quad, grp;  // quad: which 32 rows of the CTA's 128; grp: which column group
     int row;              // of the pair's tile
     uint8_t* xpose;       // its warp's bytes for transposes
-    int meetings;         // Op's own, 0 at the start: how often the warps of this quad have met
+    int meetings;         // how often the warps of this quad have met
 };
 
 struct Ring {
     uint64_t full[6], empty[6], tfull[MAX_ACC], tempty[MAX_ACC], drain;
+    uint64_t meet[4];  // of each quad's warps, where an Op has them meet
     uint32_t tmem;
     int dead;
 };
@@ -315,7 +316,17 @@ struct Ctx {
     int units, unit;   // CTAs or pairs in the grid, and this one
     uint32_t rank;     // CTA's place in its pair
     int kept;          // Op's row count, read on the device
+    Ring* ring;
 };
+
+// The warps of a quad meet: what each wrote to shared memory before is there for all
+// after. False when one of them has given up.
+__device__ __forceinline__ bool meet(Lane& me, const Ctx& x) {
+    uint64_t* bar = &x.ring->meet[me.quad];
+    __syncwarp();
+    if (me.lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    return __all_sync(0xffffffffu, wait(bar, me.meetings++ & 1, x.ring));
+}
 
 // The kernel body. Op (a __grid_constant__ parameter) has
 //   SWAP                   compile-time, CG 1: not 0 where the second operand's rows lie along TMEM's
@@ -324,7 +335,8 @@ struct Ctx {
 //   CG, F8, PROMOTE, EPI   compile-time: CTAs per tile, 8-bit operands, join accumulators in registers,
 //                          epilogue warps
 //   format                 operand format of the instruction descriptor
-//   drop                   test hook: CTA 0's producer stops before this block (-1: off)
+//   drop                   test hook: CTA 0's producer stops before this block (-1: off); below -1
+//                          CTA 0's first epilogue warp leaves before its tile -2 - drop
 //   n                      columns of a tile at most
 //   status                 the device's status word
 //   prefetch()             tensor-map prefetch
@@ -336,7 +348,8 @@ struct Ctx {
 //   zero(t, me, ctx)                                    the epilogue of a tile without blocks
 //   epilogue(t, tmem, me, ctx)                          !PROMOTE
 //   group(), Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulator is
-//                          read back and joined in registers after each `group` blocks
+//                          read back and joined in registers after each `group` blocks; finish
+//                          says false where its warps did not meet
 template <typename Op>
 __device__ __forceinline__ void run(const Op& op) {
     constexpr int CG = Op::CG;
@@ -351,6 +364,7 @@ __device__ __forceinline__ void run(const Op& op) {
     ctx.rank = CG == 2 ? cluster_rank() : 0;
     ctx.units = gridDim.x / CG;
     ctx.unit = blockIdx.x / CG;
+    ctx.ring = ring;
     if (threadIdx.x == 0) {
         for (int i = 0; i < G::STAGES; ++i) {
             mbar_init(&ring->full[i], 1);
@@ -361,6 +375,7 @@ __device__ __forceinline__ void run(const Op& op) {
             mbar_init(&ring->tempty[i], Op::EPI * CG);
         }
         mbar_init(&ring->drain, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&ring->meet[i], Op::EPI / 4);
         ring->dead = 0;
         fence_mbar_init();
         op.prefetch();
@@ -491,6 +506,7 @@ __device__ __forceinline__ void run(const Op& op) {
         uint32_t buf = 0, tph = 0;
         bool ok = true;
         for (int i = 0; ok && op.tile(i, ctx, t); ++i) {
+            if (op.drop < -1 && blockIdx.x == 0 && warp == EPI_WARP0 && i == -2 - op.drop) break;
             if (t.kn == 0) {  // an empty sum: no product, no accumulator
                 op.zero(t, me, ctx);
                 continue;
@@ -511,7 +527,7 @@ __device__ __forceinline__ void run(const Op& op) {
                     });
                     if (++buf == accs) buf = 0, tph ^= 1;
                 }
-                if (ok) op.finish(acc, t, me, ctx);
+                if (ok) ok = op.finish(acc, t, me, ctx);
             } else {
                 ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                 if (!ok) break;

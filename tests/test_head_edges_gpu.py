@@ -65,3 +65,25 @@ def test_rows_that_skip_tiles(mxs, rows, left_out, vocab, d):
     for _ in range(20):
         again = mxs.ce_from_hidden(h, w, t, temperature=0.9)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("rows,tile", [(9, 0), (100, 0), (300, 0), (300, 1)])
+def test_warps_that_meet_give_up(mxs, rows, tile):
+    """One of the four warps that meet in the loss's epilogue leaves early (a test
+    hook), while its accumulators arrive as ever: the others' wait for it ends after
+    about a second, the status word says so, and the next call gives the same bits."""
+    h, w, t = operands(rows, 20000, 512, BF, seed=40)
+    before = mxs.ce_from_hidden(h, w, t)
+    torch.cuda.synchronize()
+    mxs.get_status(clear=True)
+    mxs.set_test_hooks(drop_tile=-2 - tile)
+    try:
+        mxs.ce_from_hidden(h, w, t)
+        torch.cuda.synchronize()
+    finally:
+        mxs.set_test_hooks()
+    assert mxs.get_status(clear=True) & mxs.ROW_TIMEOUT
+    after = mxs.ce_from_hidden(h, w, t)
+    torch.cuda.synchronize()
+    assert mxs.get_status(clear=True) == 0
+    assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
