@@ -26,6 +26,7 @@
 // clock near 1.4 GHz), by the weight's bytes below.
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -85,12 +86,10 @@ struct Targets {
     }
 };
 
-// A packed row among those whose targets share 32 vocabulary rows.
-struct alignas(16) Link {
-    int next;    // the next such row or -1
-    int place;   // target % 32
-    float rest;  // what the rounding of the row's target entry of G left out
-    int unused;
+// The packed rows whose target is one vocabulary row: the first and the last of them
+// (none: first > last).
+struct alignas(8) Span {
+    int first, last;
 };
 
 struct Pack {
@@ -106,7 +105,7 @@ struct Pack {
     int* target;        // [packed]
     float* lse2;        // [packed] lse * log2(e)
     float* ghat;        // [packed] grad / gmax
-    int* first;         // [vocab / 32]: set to -1 for link_rows_kernel
+    Span* spans;        // [vocab]: emptied for GradLogitsOp (null: no gradient of the weight)
 };
 
 constexpr int PACK_T = 256;
@@ -197,9 +196,8 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
         }
     }
     if (p.grad) {
-        for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; i < (p.targets.vocab + 31) / 32;
-             i += (int64_t)gridDim.x * PACK_T)
-            p.first[i] = -1;
+        for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; p.spans && i < p.targets.vocab; i += (int64_t)gridDim.x * PACK_T)
+            p.spans[i] = Span{INT_MAX, -1};
         const int64_t words = (int64_t)((64 - all % 64) % 64) * p.ldk / STEP;  // ldk is a multiple of 8
         uint4* tail = reinterpret_cast<uint4*>(static_cast<T*>(p.packed) + (int64_t)all * p.ldk);
         for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; i < words; i += (int64_t)gridDim.x * PACK_T)
@@ -208,30 +206,6 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
     if (r1 == p.rows && r0 < r1 && tid == 0) {  // the range that ends the rows knows how many were kept
         p.head->kept = base;
         p.head->gmax = gm;
-    }
-}
-
-// The rows whose targets share 32 vocabulary rows, as chains in ascending order
-// (first[target / 32], then next): a warp a row looks through all targets.
-__global__ void __launch_bounds__(256) link_rows_kernel(const Head* head, const int* target, int* first, Link* link) {
-    mxs::gemm::grid_wait();
-    mxs::gemm::grid_launch_dependents();
-    const int lane = threadIdx.x & 31, r = blockIdx.x * 8 + (threadIdx.x >> 5), kept = head->kept;
-    if (r >= kept) return;
-    const int b = target[r] >> 5;
-    bool before = false;
-    int after = -1;
-#pragma unroll 4
-    for (int i = 0; i < kept; i += 32) {
-        const int at = i + lane;
-        const bool same = at < kept && target[at] >> 5 == b;
-        before |= __any_sync(0xffffffffu, same && at < r);
-        const uint32_t later = __ballot_sync(0xffffffffu, same && at > r);
-        if (after < 0 && later) after = i + __ffs(later) - 1;
-    }
-    if (lane == 0) {
-        link[r] = Link{after, target[r] & 31, 0.0f, 0};
-        if (!before) first[b] = r;
     }
 }
 
@@ -465,13 +439,15 @@ __global__ void __launch_bounds__(1024) score_join_kernel(const float2* part, co
 // entry outweighs the others, and its rounding would be an error common to the
 // whole row, so what it leaves out is kept in fp32 and added to both gradients
 // where they are finished (errors against 64 bits of bf16 gradients with weights of
-// all sizes: 0.0024 without, 0.0018 with, 0.0017 for the result's own rounding).
+// all sizes: 0.0024 without, 0.0018 with, 0.0017 for the result's own rounding). The
+// first and last row that leave something are kept for each target.
 // Rows after the last kept one and columns after the piece read zero.
 template <int CG_, typename T>
 struct GradLogitsOp : LogitTiles<CG_> {
     const float *lse2, *ghat;
     T* g;
-    Link* link;   // rest: what the rounding of each row's target entry leaves out
+    float* rest;  // [packed]: what the rounding of each row's target entry leaves out
+    Span* spans;  // null: no gradient of the weight
     int ldg;
     float gscale;
 
@@ -492,12 +468,19 @@ struct GradLogitsOp : LogitTiles<CG_> {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->c, -l2)) * gr;
             if (hit >= c0 && hit < c0 + 32) {
+                float left = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     if (mxs::gemm::is_column(hit - c0, j)) {
                         v[j] -= gr;
-                        link[r].rest = v[j] - to_f32(mxs::from_f32<T>(v[j]));
+                        left = v[j] - to_f32(mxs::from_f32<T>(v[j]));
                     }
+                rest[r] = left;
+                if (spans && left != 0.0f) {  // whole numbers: the same whatever the order
+                    Span* span = spans + this->v0 + t.n0 + hit;
+                    atomicMin(&span->first, r);
+                    atomicMax(&span->last, r);
+                }
             }
             if (!live || c0 + 32 > cols) {
 #pragma unroll
@@ -508,6 +491,105 @@ struct GradLogitsOp : LogitTiles<CG_> {
         }
     }
 };
+
+// What the rests of rows that share a target add to its grad_weight row:
+// sums[first] = sum_r rest_r hidden_r. (A target of one row needs none of this: the
+// product's epilogue adds that row's.) A CTA takes every gridDim.x-th vocabulary row of
+// the piece, so that neighbouring ones, which in a tokeniser's vocabulary are the
+// frequent ones, go to different CTAs, and 128 columns; its 16 warps look through the
+// targets from the first to the last row, a share each, four rows a lane, list what they
+// find in shared memory and add it, eight rows' loads in flight; the shares are added in
+// order. Bound by the latency of those reads.
+constexpr int SUM_WARPS = 16, SUM_COLS = 128, SUM_EACH = 128, SUM_LIST = SUM_EACH + 32;
+template <typename T>
+__global__ void __launch_bounds__(SUM_WARPS * 32, 2)
+    target_sums_kernel(const Span* spans, int v0, int width, const int* target, const float* rest, const T* h, int ldh,
+                       int d, float* sums, int64_t lds) {
+    mxs::gemm::grid_wait();
+    mxs::gemm::grid_launch_dependents();
+    __shared__ float4 s_part[SUM_WARPS][32];
+    __shared__ int2 s_rows[SUM_WARPS][SUM_LIST];  // row, rest
+    __shared__ Span s_spans[SUM_WARPS * 32];
+    __shared__ int s_list[SUM_WARPS * 32], s_n;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t below = (1u << lane) - 1;
+    int2* rows = s_rows[warp];
+    for (int64_t k = blockIdx.x; k < width; k += (int64_t)gridDim.x * SUM_WARPS * 32) {
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        const int64_t mine = k + (int64_t)tid * gridDim.x;
+        if (mine < width) {
+            const Span p = spans[v0 + mine];
+            if (p.first < p.last) {  // listed in any order: each stands by itself
+                const int at = atomicAdd(&s_n, 1);
+                s_list[at] = v0 + (int)mine;
+                s_spans[at] = p;
+            }
+        }
+        __syncthreads();
+        const int n = s_n;
+        for (int j = 0; j < n; ++j) {
+            const int v = s_list[j];
+            const Span p = s_spans[j];
+            const int r0 = p.first / SUM_EACH * SUM_EACH, blocks = (p.last - r0) / SUM_EACH + 1;
+            const int per = (blocks + SUM_WARPS - 1) / SUM_WARPS, b1 = min(blocks, (warp + 1) * per);
+            for (int64_t c0 = (int64_t)blockIdx.y * SUM_COLS; c0 < d; c0 += (int64_t)gridDim.y * SUM_COLS) {
+                const int64_t c = c0 + lane * 4;
+                const bool there = c < ldh;  // rows are whole 16-byte pieces
+                const T* from = h + (there ? c : 0);
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                int found = 0;
+                for (int b = warp * per; b < b1; ++b) {
+                    const int4 q = reinterpret_cast<const int4*>(target + r0 + b * SUM_EACH)[lane];
+                    const int r = r0 + b * SUM_EACH + 4 * lane, at[4] = {q.x, q.y, q.z, q.w};
+                    bool hit[4];
+                    int to = found;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        hit[i] = at[i] == v && r + i <= p.last;
+                        const uint32_t m = __ballot_sync(0xffffffffu, hit[i]);
+                        to += __popc(m & below);
+                        found += __popc(m);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (hit[i]) rows[to++] = make_int2(r + i, __float_as_int(rest[r + i]));
+                    if (found <= SUM_LIST - SUM_EACH && b + 1 < b1) continue;
+                    __syncwarp();
+                    for (int e = 0; e < found; e += 8) {
+                        uint2 u[8];
+                        float f[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int2 row = rows[min(e + i, found - 1)];
+                            f[i] = e + i < found ? __int_as_float(row.y) : 0.0f;
+                            u[i] = *reinterpret_cast<const uint2*>(from + (int64_t)row.x * ldh);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const T* x = reinterpret_cast<const T*>(&u[i]);
+                            a.x = fmaf(f[i], to_f32(x[0]), a.x);
+                            a.y = fmaf(f[i], to_f32(x[1]), a.y);
+                            a.z = fmaf(f[i], to_f32(x[2]), a.z);
+                            a.w = fmaf(f[i], to_f32(x[3]), a.w);
+                        }
+                    }
+                    __syncwarp();
+                    found = 0;
+                }
+                s_part[warp][lane] = a;
+                __syncthreads();
+                if (tid < SUM_COLS && c0 + tid < d) {
+                    float s = 0.0f;
+                    for (int w = 0; w < SUM_WARPS; ++w) s += reinterpret_cast<const float*>(s_part[w])[tid];
+                    sums[(int64_t)p.first * lds + c0 + tid] = s;
+                }
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+}
 
 // Both products of a piece in one launch. kind 0: grad_hidden += G W (M rows, N
 // d_model, K the piece's columns, cut into `splits` where the tiles alone are
@@ -528,8 +610,10 @@ struct ProductOp {
     int split_width;          // the widest piece: what the number of splits goes by
     float* acc;               // sums of grad_hidden, a block of 256 x 256 per tile and split
     bool first, want_h, want_w;
-    const int* chains;        // link_rows_kernel's
-    const Link* link;
+    const Span* spans;        // GradLogitsOp's
+    const float* rest;
+    const float* sums;        // target_sums_kernel's, [first row][lds]
+    int lds;
     const T* h;               // the packed rows
     int ldh;
     T* dw;
@@ -592,37 +676,42 @@ struct ProductOp {
         const int kr = t.kind >= 0 ? v0 + k : k;
         for (int j = 0; j < n / 128; ++j) mxs::gemm::tma_load<2>(sb + j * 8192, b, c + 64 * j, kr, bar);
     }
-    // rest_r * hidden_r, columns [c, c + 32), to the vocabulary row of row r's target,
-    // for the chain of rows from r (its link `l`) on whose targets are among the warp's 32.
-    __device__ void add_rest(float (&v)[32], int r, Link l, int c, int lane) const {
-        while (r >= 0) {
-            if (l.place == lane) {
-                const T* row = h + (int64_t)r * ldh + c;
-                if (c + 32 <= ldh) {  // rows are whole 16-byte pieces; what lies past d is not stored
+    // What the target entries' roundings left out of this thread's vocabulary row, columns
+    // [c, c + 32): the one row's rest * hidden, or the sum over the rows that share it.
+    __device__ void add_rest(float (&v)[32], Span span, float left, int c) const {
+        if (span.first == span.last) {
+            const T* row = h + (int64_t)span.first * ldh + c;
+            if (c + 32 <= ldh) {  // rows are whole 16-byte pieces; what lies past d is not stored
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(row + j);
-                        const T* e = reinterpret_cast<const T*>(&u);
+                for (int j = 0; j < 32; j += 8) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(row + j);
+                    const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) v[j + q] = fmaf(l.rest, to_f32(e[q]), v[j + q]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < d) v[j] = fmaf(l.rest, to_f32(row[j]), v[j]);
+                    for (int q = 0; q < 8; ++q) v[j + q] = fmaf(left, to_f32(e[q]), v[j + q]);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < d) v[j] = fmaf(left, to_f32(row[j]), v[j]);
             }
-            r = l.next;
-            if (r >= 0) l = link[r];
+        } else if (span.first < span.last && c < d) {  // lds is a multiple of 32
+            const float4* row = reinterpret_cast<const float4*>(sums + (int64_t)span.first * lds + c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float4 u = row[j];
+                v[4 * j] += u.x;
+                v[4 * j + 1] += u.y;
+                v[4 * j + 2] += u.z;
+                v[4 * j + 3] += u.w;
+            }
         }
         __syncwarp();
     }
     __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&) const {
         const float s = t.kind >= 0 ? 1.0f : head->gmax * scale;
         const int m = t.m0 + me.row - me.lane;  // first row of the warp
-        // pieces and tiles begin at multiples of 32 vocabulary rows
-        const int chain = t.kind >= 0 || m >= width ? -1 : chains[(v0 + m) / 32];
-        const Link head_link = chain >= 0 ? link[chain] : Link{};
+        const Span span = t.kind < 0 && m + me.lane < width ? spans[v0 + m + me.lane] : Span{INT_MAX, -1};
+        const float left = span.first == span.last ? rest[span.first] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c0 = me.grp * 32 + i * 128;
@@ -636,7 +725,7 @@ struct ProductOp {
                 else
                     mxs::gemm::store_rows<float, true>(a, 256, v, 32, 32, true, me);
             } else {
-                add_rest(v, chain, head_link, t.n0 + c0, me.lane);
+                add_rest(v, span, left, t.n0 + c0);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] *= s;
                 mxs::gemm::store_rows<T, false>(dw + (int64_t)(v0 + m) * lddw + t.n0 + c0, lddw, v, width - m,
@@ -658,7 +747,7 @@ struct ProductOp {
 // entry's rounding left out, times the scale (rows left out: zero).
 template <typename T>
 __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, const int* pos, const Head* head,
-                                                              const int* target, const Link* link, const T* w,
+                                                              const int* target, const float* rest, const T* w,
                                                               int64_t ldw, int d, int n, int width, int units,
                                                               bool want_w, float scale, T* out, int64_t ld) {
     mxs::gemm::grid_wait();
@@ -678,7 +767,7 @@ __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, 
             v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
         }
         const T* row = w + (int64_t)target[at] * ldw + k;
-        const float left = link[at].rest;
+        const float left = rest[at];
         v.x = fmaf(left, to_f32(row[0]), v.x);
         if (k + 1 < d) v.y = fmaf(left, to_f32(row[1]), v.y);
         if (k + 2 < d) v.z = fmaf(left, to_f32(row[2]), v.z);
@@ -713,13 +802,14 @@ constexpr int64_t PIECE_BYTES = 256 << 20;
 struct Plan {
     Head* head;
     void* packed;
-    int *pos, *target, *first;
-    Link* link;
+    int *pos, *target;
+    Span* spans;
+    float *rest, *sums;
     float2* part;
     float *ytarget, *lse2, *ghat, *acc;
     void* g;
     void* w;          // the weight in aligned rows, if its own are not
-    int ldk;
+    int ldk, lds;
     int n, nt;        // logit tiles
     int span;         // one tile of rows: columns of a CTA
     bool direct;      // forward on the caller's own rows
@@ -751,7 +841,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     pl.head = c.take<Head>(1);
     pl.packed = c.take<uint16_t>((size_t)rp * pl.ldk);
     pl.pos = c.take<int>(rows);
-    pl.target = c.take<int>(rows);
+    pl.target = c.take<int>(round_up(rows, 128));  // read 128 at a time
     pl.w = mxs::aligned16(weight, 2 * ldw) ? nullptr : c.take<uint16_t>((size_t)vocab * pl.ldk);
     if (!backward) {
         plan_tiles(pl, sms, rows, vocab);
@@ -760,8 +850,10 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     } else {
         pl.lse2 = c.take<float>(rows);
         pl.ghat = c.take<float>(rows);
-        pl.first = c.take<int>(ceil_div(vocab, 32));
-        pl.link = c.take<Link>(rows);
+        pl.spans = c.take<Span>(vocab);
+        pl.rest = c.take<float>(rows);
+        pl.lds = (int)round_up(d, 32);
+        pl.sums = c.take<float>((size_t)rows * pl.lds);
         const int64_t most = std::max<int64_t>(256, PIECE_BYTES / (2 * rp));
         pl.piece = round_up(ceil_div(vocab, ceil_div(vocab, most)), 256);
         plan_tiles(pl, sms, rows, std::min(pl.piece, vocab));
@@ -818,11 +910,12 @@ struct Call {
     } while (0)
 
 template <typename T>
-int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad) {
+int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad, bool want_w) {
     const Pack p{a.hidden, a.ldh, a.targets, (int)a.rows, (int)a.d, pl.ldk, lse, grad, pl.head,
-                 pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat, pl.first};
-    MXS_TRY(launch_dependent(pack_rows_kernel<T>, (unsigned)std::min<int64_t>(ceil_div(a.rows, 4), a.sms * 4), PACK_T,
-                             a.st, p));
+                 pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat, want_w ? pl.spans : nullptr};
+    // a CTA for four rows, and for 2048 spans to be emptied
+    const int64_t ctas = std::max(ceil_div(a.rows, 4), want_w ? ceil_div(a.vocab, 8 * PACK_T) : 0);
+    MXS_TRY(launch_dependent(pack_rows_kernel<T>, (unsigned)std::min<int64_t>(ctas, a.sms * 4), PACK_T, a.st, p));
     return MXS_OK;
 }
 
@@ -880,13 +973,21 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     op.lse2 = pl.lse2;
     op.ghat = pl.ghat;
     op.g = static_cast<T*>(pl.g);
-    op.link = pl.link;
+    op.rest = pl.rest;
+    op.spans = prod.want_w ? pl.spans : nullptr;
     op.ldg = (int)pl.piece;
     // f16 holds G times 2^14: the target's entry stays below its largest value
     // and entries down to 2^-28 of the largest gradient weight stay normal numbers
     op.gscale = format_of<T>() == 0 ? 16384.0f : 1.0f;
     const int64_t units = CG == 1 ? ceil_div(op.vocab, pl.span) : ceil_div(a.rows, 256) * op.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
+    if (prod.want_w) {
+        const int64_t chunks = std::min<int64_t>(ceil_div(a.d, SUM_COLS), 65535);
+        const int64_t each = std::min<int64_t>(op.vocab, std::max<int64_t>(1, 2 * a.sms / chunks));
+        MXS_TRY(launch_dependent(target_sums_kernel<T>, dim3((unsigned)each, (unsigned)chunks), SUM_WARPS * 32, a.st,
+                                 pl.spans, (int)v0, op.vocab, pl.target, pl.rest, static_cast<const T*>(pl.packed), pl.ldk,
+                                 (int)a.d, pl.sums, pl.lds));
+    }
     prod.v0 = (int)v0;
     prod.width = op.vocab;
     prod.first = v0 == 0;
@@ -910,7 +1011,7 @@ int forward(const Call& a, Plan pl, float* loss, float* lse) {
     // aligned they are read as they lie (rows left out compute numbers nobody reads).
     pl.direct = a.rows <= 128 && mxs::aligned16(a.hidden, 2 * a.ldh);
     if (!pl.direct)
-        if (const int rc = pack_rows<T>(a, pl, nullptr, nullptr)) return rc;
+        if (const int rc = pack_rows<T>(a, pl, nullptr, nullptr, false)) return rc;
     return a.rows > 128 ? score<2, T>(a, pl, w, ldw, loss, lse) : score<1, T>(a, pl, w, ldw, loss, lse);
 }
 
@@ -923,11 +1024,8 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
         MXS_TRY(mxs::copy_rows(a.weight, 2 * a.ldw, pl.w, 2 * pl.ldk, a.vocab, 2 * a.d, a.sms, a.st));
         w = pl.w, ldw = pl.ldk;
     }
-    int rc = pack_rows<T>(a, pl, lse, grad);
+    int rc = pack_rows<T>(a, pl, lse, grad, gw != nullptr);
     if (rc) return rc;
-    if (gw)  // without it the links hold `rest` alone
-        MXS_TRY(launch_dependent(link_rows_kernel, (unsigned)ceil_div(a.rows, 8), 256, a.st, pl.head, pl.target,
-                                 pl.first, pl.link));
     ProductOp<T> prod{};
     prod.format = format_of<T>();
     prod.drop = mxs::test_drop_tile();
@@ -938,8 +1036,10 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
     prod.nt = pl.dnt;
     prod.split_width = (int)std::min(pl.piece, a.vocab);
     prod.acc = pl.acc;
-    prod.chains = pl.first;
-    prod.link = pl.link;
+    prod.spans = pl.spans;
+    prod.rest = pl.rest;
+    prod.sums = pl.sums;
+    prod.lds = pl.lds;
     prod.h = static_cast<const T*>(pl.packed);
     prod.ldh = pl.ldk;
     prod.want_h = gh != nullptr;
@@ -958,7 +1058,7 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
     for (int64_t r = 0; gh && r < a.rows; r += 65535) {  // as many rows as a grid counts
         const dim3 grid((unsigned)ceil_div(a.d, 512), (unsigned)std::min<int64_t>(65535, a.rows - r));
         MXS_TRY(launch_dependent(grad_hidden_out_kernel<T>, grid, 128, a.st, pl.acc, pl.pos + r, pl.head, pl.target,
-                                 pl.link, static_cast<const T*>(w), ldw, (int)a.d, pl.dn, prod.split_width, a.sms / 2,
+                                 pl.rest, static_cast<const T*>(w), ldw, (int)a.d, pl.dn, prod.split_width, a.sms / 2,
                                  prod.want_w, prod.scale, static_cast<T*>(gh) + r * ldgh, ldgh));
     }
     return MXS_OK;

@@ -87,3 +87,83 @@ def test_warps_that_meet_give_up(mxs, rows, tile):
     torch.cuda.synchronize()
     assert mxs.get_status(clear=True) == 0
     assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
+
+
+def repeated(kind, rows, vocab, g):
+    """Targets as tokens have them: some far more often than others."""
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    if kind == "one":
+        t[:] = vocab // 2
+    elif kind == "most":
+        t[torch.rand(rows, generator=g, device="cuda") < 0.6] = vocab - 1
+    elif kind == "neighbours":
+        t %= 32
+    elif kind == "zipf":
+        p = 1.0 / torch.arange(1, vocab + 1, device="cuda", dtype=torch.float64)
+        t = torch.multinomial(p, rows, replacement=True, generator=g)
+    elif kind == "runs":  # each target's rows side by side
+        t = torch.arange(rows, device="cuda") * 7 // max(rows, 7) * (vocab // 7)
+    return t
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs"])
+@pytest.mark.parametrize("rows,vocab,d", [(2, 300, 9), (130, 1000, 200), (700, 513, 264), (2500, 4001, 72)])
+def test_repeated_targets(mxs, rows, vocab, d, kind, dt):
+    g = gen(rows + vocab)
+    h, w, _ = operands(rows, vocab, d, dt, seed=rows)
+    t = repeated(kind, rows, vocab, g)
+    grad = torch.randn(rows, generator=g, device="cuda")
+    grad[torch.rand(rows, generator=g, device="cuda") < 0.2] = 0  # rows without weight repeat too
+    _, lse, gh, gw = check_ce(mxs, h, w, t, 1.0, grad)
+    for _ in range(3):
+        again = mxs.ce_from_hidden_backward(h, w, t, lse, grad)
+        assert torch.equal(again[0], gh) and torch.equal(again[1], gw)
+
+
+@pytest.mark.parametrize("dt,vocab", [(BF, 512), (HF, 4096)])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "uniform"])
+@pytest.mark.parametrize("rows,d", [(90, 33), (1000, 300)])
+def test_target_entries_keep_32_bits(mxs, rows, d, kind, dt, vocab):
+    """A weight of zeros makes every probability 1 / vocab, a power of two, which the
+    type holds, and every target entry 1 / vocab - 1, which it does not: the weight's
+    gradient is then the formula's, rounded once (fp32 sums are within 2^-16 of it, so
+    that two elements in a hundred at most lie next to a midpoint), if and only if
+    what the entries' rounding leaves out is added for every row."""
+    g = gen(rows + vocab)
+    h = (torch.rand((rows, d), generator=g, device="cuda") + 0.5).to(dt)
+    w = torch.zeros((vocab, d), dtype=dt, device="cuda")
+    t = repeated(kind, rows, vocab, g)
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    _, gw = mxs.ce_from_hidden_backward(h, w, t, lse, torch.ones(rows, device="cuda"), need_hidden=False)
+    def gradient(entry):
+        dw = (h.double().sum(0) / vocab).repeat(vocab, 1)
+        return dw.index_add_(0, t, h.double() * (entry - 1 / vocab))
+    want, hit = gradient(1 / vocab - 1), torch.unique(t)
+    rounded = torch.tensor(1 / vocab - 1, dtype=dt, device="cuda").double().item()
+    wrong = gradient(rounded)[hit].to(dt) != want[hit].to(dt)
+    assert wrong.float().mean() > 0.1  # without the rests
+    assert (gw != want.to(dt)).float().mean() <= 0.02
+    assert (gw[hit] != want[hit].to(dt)).float().mean() <= 0.02
+    u = head_ref.U[dt]
+    assert ((gw.double() - want).abs() <= (u + 2.0 ** -16) * want.abs() + 2.0 ** -25).all()
+
+
+def test_a_million_rows_of_one_target(mxs):
+    """Padding that keeps its token id and its weight: no wait runs out, and the time is
+    the products'. fp32 sums of so many products of one sign lose up to 2^-23 of
+    themselves at every 16 of them."""
+    rows, vocab, d = 1200000, 512, 8
+    g = gen(1)
+    h = (torch.rand((rows, d), generator=g, device="cuda") + 0.5).to(BF)
+    w = torch.zeros((vocab, d), dtype=BF, device="cuda")
+    t = torch.full((rows,), 77, device="cuda")
+    t[::1000] = 78
+    mxs.get_status(clear=True)
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    _, gw = mxs.ce_from_hidden_backward(h, w, t, lse, torch.ones(rows, device="cuda"), need_hidden=False)
+    torch.cuda.synchronize()
+    assert mxs.get_status(clear=True) == 0
+    want = (h.double().sum(0) / vocab).repeat(vocab, 1).index_add_(0, t, -h.double())
+    size = (h.double().sum(0) / vocab).repeat(vocab, 1).index_add_(0, t, h.double())
+    assert ((gw.double() - want).abs() <= 2.0 ** -8 * want.abs() + rows / 16 * 2.0 ** -23 * size).all()
