@@ -167,3 +167,91 @@ def test_a_million_rows_of_one_target(mxs):
     want = (h.double().sum(0) / vocab).repeat(vocab, 1).index_add_(0, t, -h.double())
     size = (h.double().sum(0) / vocab).repeat(vocab, 1).index_add_(0, t, h.double())
     assert ((gw.double() - want).abs() <= 2.0 ** -8 * want.abs() + rows / 16 * 2.0 ** -23 * size).all()
+
+
+# ---------------------------------------------------------------------------
+# Several pieces of the vocabulary, real heads' widths
+# ---------------------------------------------------------------------------
+
+def ceil_div(a, b):
+    return -(-a // b)
+
+
+def piece_of(rows, vocab):
+    """Columns of a piece of the gradients (make_plan in mxs_ce.cu: 256 MB of G)."""
+    most = max(256, (256 << 20) // (2 * ceil_div(rows, 256) * 256))
+    return ceil_div(ceil_div(vocab, ceil_div(vocab, most)), 256) * 256
+
+
+def in_pieces(mxs, rows, vocab, d, dt, seed, pieces):
+    """operands() with targets on both sides of every piece's edge and in the last rows of
+    the vocabulary; that G is not held whole shows in the workspace's size."""
+    import ctypes
+    piece = piece_of(rows, vocab)
+    assert ceil_div(vocab, piece) == pieces
+    h, w, t = operands(rows, vocab, d, dt, seed=seed)
+    need = ctypes.c_size_t()
+    assert mxs.load().mxs_ce_workspace_size(ctypes.c_void_p(w.data_ptr()), w.stride(0), rows, d, vocab, 1,
+                                            ctypes.byref(need)) == 0
+    if rows * d < 1 << 20:  # else the rows' own scratch hides it
+        assert need.value < 2 * ceil_div(rows, 256) * 256 * vocab
+    at = [0, vocab - 1, vocab - 2, vocab - 31, vocab - 33]
+    for p in range(1, pieces):
+        at += [p * piece - 33, p * piece - 2, p * piece - 1, p * piece, p * piece + 1, p * piece + 32]
+    t[:2 * len(at)] = torch.tensor(at * 2, device="cuda")  # each twice
+    t[rows // 2] = -100
+    return h, w, t
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("rows,vocab,d,pieces", [(4000, 40001, 24, 2), (4000, 40001, 264, 2), (4000, 70001, 72, 3),
+                                                 (1500, 200003, 40, 3), (300, 600001, 16, 3), (128, 1100001, 8, 3)])
+def test_gradients_in_several_pieces(mxs, rows, vocab, d, pieces, dt):
+    check_ce(mxs, *in_pieces(mxs, rows, vocab, d, dt, rows + d, pieces), 0.9)
+
+
+def hidden_splits(rows, nt, width, units):
+    """Splits of K for grad_hidden alone (grad_hidden_splits in mxs_ce.cu)."""
+    tiles, blocks = ceil_div(rows, 256) * nt, ceil_div(width, 64)
+    s = max(1, min(ceil_div(blocks * units, tiles * blocks), ceil_div(blocks, 8), units // tiles))
+    return ceil_div(blocks, ceil_div(blocks, s))
+
+
+@pytest.mark.parametrize("need", ["hidden", "weight"])
+@pytest.mark.parametrize("rows,vocab,d", [(130, 533024, 8), (130, 541759, 200), (2000, 140000, 40)])
+def test_one_gradient_in_several_pieces(mxs, rows, vocab, d, need):
+    """One gradient alone; for 130 rows the last, narrower piece leaves the last split of
+    grad_hidden's sum without a column."""
+    h, w, t = in_pieces(mxs, rows, vocab, d, BF, 3, ceil_div(vocab, piece_of(rows, vocab)))
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    if rows == 130 and pairs == 74:
+        piece, last = piece_of(rows, vocab), vocab % piece_of(rows, vocab)
+        s = hidden_splits(rows, 1, piece, pairs)
+        blocks = ceil_div(last, 64)
+        assert (s - 1) * ceil_div(blocks, s) >= blocks
+    grad = torch.randn(rows, generator=gen(9), device="cuda")
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    gh, gw = mxs.ce_from_hidden_backward(h, w, t, lse, grad, need_hidden=need == "hidden",
+                                         need_weight=need == "weight")
+    dh, dw, eh, ew = head_ref.ce_grads(h, w, t, grad, 1.0)
+    got, want, tol = (gh, dh, eh) if need == "hidden" else (gw, dw, ew)
+    assert (gw if need == "hidden" else gh) is None
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("rows,vocab,d", [(130, 3001, 1100), (300, 2000, 896), (257, 1500, 3584), (520, 5000, 2048),
+                                          (700, 1999, 1037), (100, 1999, 3584)])
+def test_heads_of_real_widths(mxs, rows, vocab, d, dt):
+    """More than 128 rows with a d_model of several joins of the loss's accumulators."""
+    check_ce(mxs, *operands(rows, vocab, d, dt, seed=d), 0.9)
+
+
+@pytest.mark.parametrize("rows,n,k,out", [(65, 3000, 3584, torch.float32), (100, 5001, 1040, BF),
+                                          (128, 700, 8192, HF), (260, 3001, 3584, torch.float32),
+                                          (1000, 1024, 8192, BF)])
+def test_matmul_fp8_real_widths(mxs, rows, n, k, out):
+    ops = fp8_operands(rows, n, k, seed=k)
+    got = mxs.matmul_fp8(*ops, out_dtype=out)
+    want, tol = head_ref.matmul_fp8(*ops, out)
+    assert ((got.double() - want).abs() <= tol).all()
