@@ -255,3 +255,43 @@ def test_matmul_fp8_real_widths(mxs, rows, n, k, out):
     got = mxs.matmul_fp8(*ops, out_dtype=out)
     want, tol = head_ref.matmul_fp8(*ops, out)
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", [HF, BF])
+@pytest.mark.parametrize("wrt,step", [("hidden", 2.0 ** -5), ("weight", 2.0 ** -8)])
+@pytest.mark.parametrize("seed", [0, 1, 2, 3])
+def test_gradients_against_differences(mxs, wrt, step, seed, dt):
+    """Central differences of the kernel's own losses along a direction of 64 elements,
+    in steps that the types hold exactly. The error: the losses' own (their bounds, as a
+    random walk over the rows), a third derivative's, at most the cube of a row's
+    largest move of a logit, over 6, and the gradients' (their elementwise bounds along
+    the direction). The derivative is at least 20 times that, so that a gradient 5 % off
+    fails."""
+    rows, vocab, d = 60, 300, 32
+    g = gen(seed)
+    h = (torch.randint(-16, 17, (rows, d), generator=g, device="cuda") / 8).to(dt)
+    w = (torch.randint(-16, 17, (vocab, d), generator=g, device="cuda") / 32).to(dt)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    if seed == 3:
+        t %= 8
+    loss, lse = mxs.ce_from_hidden(h, w, t)
+    gh, gw = mxs.ce_from_hidden_backward(h, w, t, lse, torch.ones(rows, device="cuda"))
+    x, grad = (h, gh) if wrt == "hidden" else (w, gw)
+    at = torch.randperm(x.numel(), generator=g, device="cuda")[:64]
+    move = torch.zeros_like(x)
+    move.view(-1)[at] = step * grad.view(-1)[at].sign()
+    assert ((x + move).double() == x.double() + move.double()).all()
+    assert ((x - move).double() == x.double() - move.double()).all()
+    def total(sign):
+        y = x + sign * move
+        return mxs.ce_from_hidden(y if wrt == "hidden" else h, w if wrt == "hidden" else y, t)[0].double().sum().item()
+    difference = (total(1) - total(-1)) / 2
+    derivative = (grad.double() * move.double()).sum().item()
+    moved = move.double() @ w.double().t() if wrt == "hidden" else h.double() @ move.double().t()
+    cubic = (moved.abs().amax(1) ** 3).sum().item() / 6
+    _, _, eh, ew = head_ref.ce_grads(h, w, t, torch.ones(rows, device="cuda"), 1.0)
+    own = ((eh if wrt == "hidden" else ew) * move.double().abs()).sum().item()
+    tl, _ = head_ref.ce_tol(h, w, t, 1.0, *head_ref.ce(h, w, t, 1.0))
+    tol = tl.norm().item() + cubic + own
+    assert abs(difference - derivative) <= tol, (difference, derivative, tol)
+    assert abs(derivative) >= 20 * tol
