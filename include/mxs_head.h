@@ -63,7 +63,7 @@ MXS_API int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const vo
  * Both are written whole (rows left out get a zero gradient); either may be NULL
  * and is then not computed. The logits are computed again, a piece of the
  * vocabulary at a time; a piece of grad_loss_r P[r][v] / max |grad_loss| is held in
- * `dtype` (for MXS_F16 entries below 2^-28 of the largest weight lose precision),
+ * `dtype` (entries below 2^-28 (MXS_F16) or 2^-126 (MXS_BF16) lose precision),
  * what that rounding leaves out of a row's target entry is kept in fp32, sums are
  * fp32, and the gradients are rounded to `dtype` once.
  */

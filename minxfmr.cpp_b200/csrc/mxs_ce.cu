@@ -708,7 +708,8 @@ struct ProductOp {
         __syncwarp();
     }
     __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&) const {
-        const float s = t.kind >= 0 ? 1.0f : head->gmax * scale;
+        // two factors: their product may leave fp32's range where the results do not
+        const float gmax = t.kind >= 0 ? 1.0f : head->gmax;
         const int m = t.m0 + me.row - me.lane;  // first row of the warp
         const Span span = t.kind < 0 && m + me.lane < width ? spans[v0 + m + me.lane] : Span{INT_MAX, -1};
         const float left = span.first == span.last ? rest[span.first] : 0.0f;
@@ -727,7 +728,7 @@ struct ProductOp {
             } else {
                 add_rest(v, span, left, t.n0 + c0);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= s;
+                for (int j = 0; j < 32; ++j) v[j] = v[j] * scale * gmax;
                 mxs::gemm::store_rows<T, false>(dw + (int64_t)(v0 + m) * lddw + t.n0 + c0, lddw, v, width - m,
                                                 d - t.n0 - c0, vec, me);
             }
@@ -772,8 +773,8 @@ __global__ void __launch_bounds__(128) grad_hidden_out_kernel(const float* acc, 
         if (k + 1 < d) v.y = fmaf(left, to_f32(row[1]), v.y);
         if (k + 2 < d) v.z = fmaf(left, to_f32(row[2]), v.z);
         if (k + 3 < d) v.w = fmaf(left, to_f32(row[3]), v.w);
-        const float s = head->gmax * scale;
-        v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
+        const float g = head->gmax;  // as in ProductOp
+        v = make_float4(v.x * scale * g, v.y * scale * g, v.z * scale * g, v.w * scale * g);
     }
     T* o = out + r * ld + k;
     const float y[4] = {v.x, v.y, v.z, v.w};

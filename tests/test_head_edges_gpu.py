@@ -295,3 +295,23 @@ def test_gradients_against_differences(mxs, wrt, step, seed, dt):
     tol = tl.norm().item() + cubic + own
     assert abs(difference - derivative) <= tol, (difference, derivative, tol)
     assert abs(derivative) >= 20 * tol
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 0.7, 3.0])
+def test_gradient_weights_near_the_largest_float(mxs, temperature):
+    """A row's gradient scales with its own weight, however large another's: zero for a
+    weight of zero, finite where the formula's is."""
+    h, w, t = operands(6, 400, 64, BF, seed=4)
+    w *= 2.0 ** -8
+    t[:] = torch.arange(6, device="cuda") * 40
+    grad = torch.tensor([0.0, 1e30, -1e20, 3.3e38, -3.3e38, 0.0], device="cuda")
+    _, lse = mxs.ce_from_hidden(h, w, t, temperature=temperature)
+    gh, gw = mxs.ce_from_hidden_backward(h, w, t, lse, grad, temperature=temperature)
+    dh, _, eh, _ = head_ref.ce_grads(h, w, t, grad, temperature)
+    assert (gh[[0, 5]] == 0).all()
+    assert (dh.abs() < 3.0e38).all() and ((gh.double() - dh).abs() <= eh).all()
+    tiny = h * 2.0 ** -8  # the weight's gradient stays in range too
+    _, lse = mxs.ce_from_hidden(tiny, w, t, temperature=temperature)
+    _, gw = mxs.ce_from_hidden_backward(tiny, w, t, lse, grad, temperature=temperature)
+    _, dw, _, ew = head_ref.ce_grads(tiny, w, t, grad, temperature)
+    assert (dw.abs() < 3.0e38).all() and ((gw.double() - dw).abs() <= ew).all()
