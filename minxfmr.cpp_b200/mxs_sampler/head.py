@@ -42,6 +42,8 @@ def _on(dev, stream):
     """The device and stream of a call made current, where they are not."""
     if stream is None and dev == torch.cuda.current_device():
         return _HERE
+    if stream is not None and stream.device_index != dev:
+        raise ValueError(f"stream is on cuda:{stream.device_index}, the operands on cuda:{dev}")
     return _elsewhere(dev, stream)
 
 
