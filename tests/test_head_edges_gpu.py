@@ -315,3 +315,97 @@ def test_gradient_weights_near_the_largest_float(mxs, temperature):
     _, gw = mxs.ce_from_hidden_backward(tiny, w, t, lse, grad, temperature=temperature)
     _, dw, _, ew = head_ref.ce_grads(tiny, w, t, grad, temperature)
     assert (dw.abs() < 3.0e38).all() and ((gw.double() - dw).abs() <= ew).all()
+
+
+# ---------------------------------------------------------------------------
+# 8 bits: layouts, graphs, arguments
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("out", [torch.float32, BF, HF])
+@pytest.mark.parametrize("rows", [1, 20, 61, 100, 150, 300])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 0), (11, 1), (8, 8)])
+def test_matmul_fp8_output_layouts(mxs, rows, pad, offset, out):
+    """Every kernel's stores, into rows of any alignment; nothing is written between them."""
+    ops = fp8_operands(rows, 301, 200, seed=rows)
+    flat = torch.full((rows * (301 + pad) + offset,), -7.0, dtype=out, device="cuda")
+    view = flat[offset:].view(rows, 301 + pad)
+    mxs.matmul_fp8(*ops, out=view[:, :301])
+    want, tol = head_ref.matmul_fp8(*ops, out)
+    assert ((view[:, :301].double() - want).abs() <= tol).all()
+    assert (view[:, 301:] == -7.0).all() and (flat[:offset] == -7.0).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 140])
+@pytest.mark.parametrize("d,pad", [(200, 0), (208, 0), (99, 13)])
+def test_sample_from_hidden_fp8_layouts(mxs, rows, d, pad):
+    """Weights and logits with rows of any alignment: the same logits and draws."""
+    g = gen(rows + d)
+    vocab = 3001
+    h = torch.randn((rows, d), generator=g, device="cuda").to(BF)
+    wq, ws = mxs.quantize_fp8((torch.randn((vocab, d), generator=g, device="cuda") * (3 / d ** 0.5)).to(BF), 128)
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    loose = torch.empty((vocab, d + pad), dtype=torch.uint8, device="cuda")[:, :d].view(torch.float8_e4m3fn)
+    loose.copy_(wq)
+    want = mxs.matmul_fp8(*mxs.quantize_fp8(h, 1), wq, ws)
+    n0, i0, p0 = mxs.sample(want, 0.8, 40, u)
+    for extra in (None, 0, 5):
+        logits = None if extra is None else torch.empty((rows, vocab + extra), device="cuda")[:, :vocab]
+        n, i, p = mxs.sample_from_hidden_fp8(h, loose, ws, 0.8, 40, u, logits_out=logits)
+        assert torch.equal(n, n0) and torch.equal(i, i0) and torch.equal(p, p0)
+        assert logits is None or torch.equal(logits, want)
+
+
+@pytest.mark.parametrize("rows", [1, 33, 200])
+def test_fp8_calls_in_a_graph(mxs, rows):
+    """Quantiser, product and draw captured, and replayed on other hidden states; and on
+    a stream of their own."""
+    g = gen(rows)
+    vocab, d = 5000, 384
+    h = torch.randn((rows, d), generator=g, device="cuda").to(HF)
+    wq, ws = mxs.quantize_fp8((torch.randn((vocab, d), generator=g, device="cuda") * 0.15).to(HF), 128)
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    def step(stream=None):
+        q, s = mxs.quantize_fp8(h, 1, stream=stream)
+        return (mxs.matmul_fp8(q, s, wq, ws, out_dtype=BF, stream=stream),) + mxs.sample_from_hidden_fp8(
+            h, wq, ws, 1.1, 20, u, stream=stream)
+    first = step()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    other = step(side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    h.copy_(torch.randn((rows, d), generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_fp8_draws_of_no_rows(mxs):
+    wq, ws = mxs.quantize_fp8(torch.ones((50, 64), dtype=BF, device="cuda"), 128)
+    h = torch.empty((0, 64), dtype=BF, device="cuda")
+    n, i, p = mxs.sample_from_hidden_fp8(h, wq, ws, 1.0, 5, torch.empty(0, dtype=torch.float64, device="cuda"))
+    assert n.shape == (0,) and i.shape == (0, 5) and p.shape == (0, 5)
+
+
+@pytest.mark.parametrize("rows", [9, 300])
+def test_loss_or_lse_alone(mxs, rows):
+    """Either output of the C call may be left out."""
+    import ctypes
+    P = ctypes.c_void_p
+    h, w, t = operands(rows, 700, 96, BF, seed=rows)
+    loss, lse = mxs.ce_from_hidden(h, w, t)
+    need = ctypes.c_size_t()
+    lib = mxs.load()
+    assert lib.mxs_ce_workspace_size(P(w.data_ptr()), 96, rows, 96, 700, 0, ctypes.byref(need)) == 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    for which in (0, 1):
+        out = torch.full((rows,), -1.0, device="cuda")
+        at = [P(out.data_ptr()), None] if which == 0 else [None, P(out.data_ptr())]
+        torch.cuda.synchronize()
+        assert lib.mxs_ce_from_hidden(P(h.data_ptr()), 96, P(w.data_ptr()), 96, 0, rows, 96, 700, P(t.data_ptr()), 8,
+                                      1.0, *at, P(ws.data_ptr()), need.value, None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, loss if which == 0 else lse)
