@@ -45,6 +45,9 @@ using mxs::gemm::Lane;
 using mxs::gemm::Tile;
 
 constexpr int64_t MAX_DIM = INT32_MAX - 1024;
+// grad_weight sums over the rows in one run of products, 512 clocks at least for each
+// 64: 2^26 rows take 0.3 to 0.5 s of the second that their end is waited for.
+constexpr int64_t MAX_BACKWARD_ROWS = 1 << 26;
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.4426950408889634074;
 
@@ -1072,7 +1075,7 @@ extern "C" {
 int mxs_ce_workspace_size(const void* d_weight, int64_t ld_weight, int64_t rows, int64_t d_model, int64_t vocab,
                           int backward, size_t* bytes) {
     if (!bytes || rows < 0 || d_model <= 0 || vocab <= 0 || ld_weight < d_model || rows > MAX_DIM ||
-        d_model > MAX_DIM || vocab > MAX_DIM)
+        d_model > MAX_DIM || vocab > MAX_DIM || (backward && rows > MAX_BACKWARD_ROWS))
         return MXS_ERR_INVALID;
     int sms = 0;
     uint32_t* status = nullptr;
@@ -1104,7 +1107,8 @@ int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const v
                                 void* d_grad_hidden, int64_t ld_grad_hidden, void* d_grad_weight,
                                 int64_t ld_grad_weight, void* d_workspace, size_t workspace_bytes, void* stream) {
     if (bad_shape(ld_hidden, ld_weight, dtype, rows, d_model, vocab, target_bytes, temperature) ||
-        (d_grad_hidden && ld_grad_hidden < d_model) || (d_grad_weight && ld_grad_weight < d_model))
+        rows > MAX_BACKWARD_ROWS || (d_grad_hidden && ld_grad_hidden < d_model) ||
+        (d_grad_weight && ld_grad_weight < d_model))
         return MXS_ERR_INVALID;
     if (!d_grad_hidden && !d_grad_weight) return MXS_OK;
     Call a{d_hidden, ld_hidden, d_weight, ld_weight, rows, d_model, vocab,
