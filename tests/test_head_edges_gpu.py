@@ -101,13 +101,17 @@ def repeated(kind, rows, vocab, g):
     elif kind == "zipf":
         p = 1.0 / torch.arange(1, vocab + 1, device="cuda", dtype=torch.float64)
         t = torch.multinomial(p, rows, replacement=True, generator=g)
+    elif kind == "counts":  # groups of 1, 2, ... rows on either side of 16, in any order
+        sizes = torch.tensor([1, 2, 3, 15, 16, 17, 18, 33] * (rows // 105 + 1), device="cuda")
+        t = (torch.arange(len(sizes), device="cuda") * 5 % vocab).repeat_interleave(sizes)[:rows]
+        t = t[torch.randperm(rows, generator=g, device="cuda")]
     elif kind == "runs":  # each target's rows side by side
         t = torch.arange(rows, device="cuda") * 7 // max(rows, 7) * (vocab // 7)
     return t
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
-@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs"])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts"])
 @pytest.mark.parametrize("rows,vocab,d", [(2, 300, 9), (130, 1000, 200), (700, 513, 264), (2500, 4001, 72)])
 def test_repeated_targets(mxs, rows, vocab, d, kind, dt):
     g = gen(rows + vocab)
@@ -122,7 +126,7 @@ def test_repeated_targets(mxs, rows, vocab, d, kind, dt):
 
 
 @pytest.mark.parametrize("dt,vocab", [(BF, 512), (HF, 4096)])
-@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "uniform"])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts", "uniform"])
 @pytest.mark.parametrize("rows,d", [(90, 33), (1000, 300)])
 def test_target_entries_keep_32_bits(mxs, rows, d, kind, dt, vocab):
     """A weight of zeros makes every probability 1 / vocab, a power of two, which the
@@ -409,3 +413,18 @@ def test_loss_or_lse_alone(mxs, rows):
                                       1.0, *at, P(ws.data_ptr()), need.value, None) == 0
         torch.cuda.synchronize()
         assert torch.equal(out, loss if which == 0 else lse)
+
+
+def test_f16_gradient_weights_of_many_sizes(mxs):
+    """f16 holds entries relative to the largest weight: down to 2^-28 of it as exactly as
+    ever, below with an absolute error that the bound has."""
+    h, w, t = operands(120, 900, 72, HF, seed=14)
+    grad = torch.exp2(-torch.arange(120, device="cuda") / 3) * 3e3  # down to 2^-40 of the largest
+    grad[::2] *= -1
+    check_ce(mxs, h, w, t, 1.0, grad)
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    for scale in (2.0 ** -12, 2.0 ** 3):  # the division by the largest weight is exact for powers of two
+        a = mxs.ce_from_hidden_backward(h, w, t, lse, grad)[0]
+        b = mxs.ce_from_hidden_backward(h, w, t, lse, grad * scale)[0]
+        ok = (a.abs() >= 2.0 ** -2) & (b.abs() >= 2.0 ** -13)  # both in f16's normal range
+        assert ok.any() and torch.equal((a.double() * scale)[ok], b.double()[ok])
