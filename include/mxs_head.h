@@ -65,7 +65,7 @@ MXS_API int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const vo
  * vocabulary at a time; a piece of grad_loss_r P[r][v] / max |grad_loss| is held in
  * `dtype` (entries below 2^-28 (MXS_F16) or 2^-126 (MXS_BF16) lose precision),
  * what that rounding leaves out of a row's target entry is kept in fp32, sums are
- * fp32, and the gradients are rounded to `dtype` once. At most 2^26 rows a call.
+ * fp32, and the gradients are rounded to `dtype` once. At most 2^24 rows a call.
  */
 MXS_API int mxs_ce_from_hidden_backward(const void* d_hidden, int64_t ld_hidden, const void* d_weight,
                                         int64_t ld_weight, int dtype, int64_t rows, int64_t d_model, int64_t vocab,

@@ -45,9 +45,10 @@ using mxs::gemm::Lane;
 using mxs::gemm::Tile;
 
 constexpr int64_t MAX_DIM = INT32_MAX - 1024;
-// grad_weight sums over the rows in one run of products, 512 clocks at least for each
-// 64: 2^26 rows take 0.3 to 0.5 s of the second that their end is waited for.
-constexpr int64_t MAX_BACKWARD_ROWS = 1 << 26;
+// What a wait of at most a second spans grows with the rows: grad_weight's run of products
+// (512 clocks at least for each 64 rows) and, where more than 16 rows share a target, the
+// looking for them (128 such targets a CTA). 2^24 rows take half of it at most.
+constexpr int64_t MAX_BACKWARD_ROWS = 1 << 24;
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.4426950408889634074;
 
@@ -90,11 +91,13 @@ struct Targets {
 };
 
 // The packed rows whose target is one vocabulary row and whose entry of G its rounding
-// changed: how many, and the one that was counted first (any of them).
-struct alignas(8) Group {
-    int count, row;
+// changed are its group: counted for every vocabulary row, and the first LISTED of them,
+// in any order, written down with what the rounding left out.
+constexpr int LISTED = 16;
+struct alignas(8) Left {
+    int row;
+    float rest;
 };
-constexpr int LISTED = 16;  // rows of a group that are written down, in any order
 
 struct Pack {
     const void* hidden;
@@ -109,7 +112,7 @@ struct Pack {
     int* target;        // [packed]
     float* lse2;        // [packed] lse * log2(e)
     float* ghat;        // [packed] grad / gmax
-    Group* groups;      // [vocab]: emptied for GradLogitsOp (null: no gradient of the weight)
+    int* counts;        // [vocab]: zeroed for GradLogitsOp (null: no gradient of the weight)
 };
 
 constexpr int PACK_T = 256;
@@ -200,9 +203,9 @@ __global__ void __launch_bounds__(PACK_T) pack_rows_kernel(const Pack p) {
         }
     }
     if (p.grad) {
-        for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; p.groups && i < p.targets.vocab;
+        for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; p.counts && i < p.targets.vocab;
              i += (int64_t)gridDim.x * PACK_T)
-            p.groups[i] = Group{0, 0};
+            p.counts[i] = 0;
         const int64_t words = (int64_t)((64 - all % 64) % 64) * p.ldk / STEP;  // ldk is a multiple of 8
         uint4* tail = reinterpret_cast<uint4*>(static_cast<T*>(p.packed) + (int64_t)all * p.ldk);
         for (int64_t i = blockIdx.x * (int64_t)PACK_T + tid; i < words; i += (int64_t)gridDim.x * PACK_T)
@@ -452,12 +455,16 @@ struct GradLogitsOp : LogitTiles<CG_> {
     const float *lse2, *ghat;
     T* g;
     float* rest;  // [packed]: what the rounding of each row's target entry leaves out
-    Group* groups;  // [vocab]; null: no gradient of the weight
-    int* listed;    // [piece][LISTED]
+    int* counts;    // [vocab]; null: no gradient of the weight
+    Left* listed;   // [piece][LISTED]
     int ldg;
     float gscale;
 
-    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x) const {
+    struct Ahead {
+        static constexpr bool ok = true;
+    };
+    __device__ Ahead ahead(const Tile&, const Lane&, const Ctx&) const { return {}; }
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x, Ahead) const {
         const int r = t.m0 + me.row;
         const bool live = r < x.kept;
         const int hit = live ? this->target[r] - this->v0 - t.n0 : -1;
@@ -482,11 +489,10 @@ struct GradLogitsOp : LogitTiles<CG_> {
                         left = v[j] - to_f32(mxs::from_f32<T>(v[j]));
                     }
                 rest[r] = left;
-                if (groups && left != 0.0f) {
+                if (counts && left != 0.0f) {
                     const int64_t v = t.n0 + hit;
-                    const int k = atomicAdd(&groups[this->v0 + v].count, 1);
-                    if (k == 0) groups[this->v0 + v].row = r;
-                    if (k < LISTED) listed[v * LISTED + k] = r;
+                    const int k = atomicAdd(counts + this->v0 + v, 1);
+                    if (k < LISTED) listed[v * LISTED + k] = Left{r, left};
                 }
             }
             if (!live || c0 + 32 > cols) {
@@ -498,131 +504,6 @@ struct GradLogitsOp : LogitTiles<CG_> {
         }
     }
 };
-
-// What the rests of rows that share a target add to its grad_weight row:
-// sums[group's row] = sum_r rest_r hidden_r, in ascending order of the rows whatever the
-// order they were counted in. (A target of one row needs none of this: the product's
-// epilogue adds that row's.) A CTA takes every gridDim.x-th vocabulary row of the piece,
-// so that neighbouring ones, which in a tokeniser's vocabulary are the frequent ones, go
-// to different CTAs, and 128 columns. A group of up to LISTED rows is a warp's: it sorts
-// the list and adds. A larger one is the CTA's: each warp looks through a sixteenth of all
-// targets, four a lane, lists what it finds and adds it; the warps' sums are added in
-// order. Eight rows' loads are in flight; bound by their latency. 4096 rows x 32000 x 512:
-// 6 us with uniform targets, 11 with Zipf ones, 43 with one; x 16384 x 3584, uniform: 15 us,
-// and 85 when every group was the CTA's.
-constexpr int SUM_WARPS = 16, SUM_COLS = 128, SUM_EACH = 128, SUM_LIST = SUM_EACH + 32;
-
-// a += rest * hidden of n listed rows, four columns from `from` on.
-template <typename T>
-__device__ __forceinline__ void add_rows(float4& a, const int2* rows, int n, const T* from, int ldh) {
-    for (int e = 0; e < n; e += 8) {
-        uint2 u[8];
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int2 row = rows[min(e + i, n - 1)];
-            f[i] = e + i < n ? __int_as_float(row.y) : 0.0f;
-            u[i] = *reinterpret_cast<const uint2*>(from + (int64_t)row.x * ldh);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const T* x = reinterpret_cast<const T*>(&u[i]);
-            a.x = fmaf(f[i], to_f32(x[0]), a.x);
-            a.y = fmaf(f[i], to_f32(x[1]), a.y);
-            a.z = fmaf(f[i], to_f32(x[2]), a.z);
-            a.w = fmaf(f[i], to_f32(x[3]), a.w);
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(SUM_WARPS * 32, 2)
-    target_sums_kernel(const Head* head, const Group* groups, const int* listed, int v0, int width, const int* target,
-                       const float* rest, const T* h, int ldh, int d, float* sums, int64_t lds) {
-    mxs::gemm::grid_wait();
-    mxs::gemm::grid_launch_dependents();
-    __shared__ float4 s_part[SUM_WARPS][32];
-    __shared__ int2 s_rows[SUM_WARPS][SUM_LIST];  // row, rest
-    __shared__ int s_few[SUM_WARPS * 32], s_many[SUM_WARPS * 32], s_n[2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kept = *(volatile const int*)&head->kept;
-    const uint32_t below = (1u << lane) - 1;
-    int2* rows = s_rows[warp];
-    for (int64_t k = blockIdx.x; k < width; k += (int64_t)gridDim.x * SUM_WARPS * 32) {
-        if (tid < 2) s_n[tid] = 0;
-        __syncthreads();
-        const int64_t mine = k + (int64_t)tid * gridDim.x;
-        if (mine < width) {
-            const int n = groups[v0 + mine].count;  // listed in any order: each group stands by itself
-            if (n > LISTED)
-                s_many[atomicAdd(&s_n[1], 1)] = (int)mine;
-            else if (n > 1)
-                s_few[atomicAdd(&s_n[0], 1)] = (int)mine;
-        }
-        __syncthreads();
-        for (int j = warp; j < s_n[0]; j += SUM_WARPS) {
-            const int v = s_few[j];
-            const Group g = groups[v0 + v];
-            const int r = lane < g.count ? listed[(int64_t)v * LISTED + lane] : INT_MAX;
-            int to = 0;
-#pragma unroll
-            for (int i = 0; i < LISTED; ++i) to += __shfl_sync(0xffffffffu, r, i) < r;
-            __syncwarp();
-            if (lane < g.count) rows[to] = make_int2(r, __float_as_int(rest[r]));
-            __syncwarp();
-            for (int64_t c0 = (int64_t)blockIdx.y * SUM_COLS; c0 < d; c0 += (int64_t)gridDim.y * SUM_COLS) {
-                const int64_t c = c0 + lane * 4;
-                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                add_rows(a, rows, g.count, h + (c < ldh ? c : 0), ldh);  // rows are whole 16-byte pieces
-                if (c < d) *reinterpret_cast<float4*>(sums + (int64_t)g.row * lds + c) = a;
-            }
-            __syncwarp();
-        }
-        const int many = s_n[1];
-        for (int j = 0; j < many; ++j) {
-            const int v = v0 + s_many[j];
-            const int64_t to_row = (int64_t)groups[v].row * lds;
-            const int blocks = (kept + SUM_EACH - 1) / SUM_EACH;
-            const int per = (blocks + SUM_WARPS - 1) / SUM_WARPS, b1 = min(blocks, (warp + 1) * per);
-            for (int64_t c0 = (int64_t)blockIdx.y * SUM_COLS; c0 < d; c0 += (int64_t)gridDim.y * SUM_COLS) {
-                const int64_t c = c0 + lane * 4;
-                const T* from = h + (c < ldh ? c : 0);
-                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                int found = 0;
-                for (int b = warp * per; b < b1; ++b) {
-                    const int4 q = reinterpret_cast<const int4*>(target + (int64_t)b * SUM_EACH)[lane];
-                    const int r = b * SUM_EACH + 4 * lane, at[4] = {q.x, q.y, q.z, q.w};
-                    bool hit[4];
-                    int to = found;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        hit[i] = at[i] == v && r + i < kept;
-                        const uint32_t m = __ballot_sync(0xffffffffu, hit[i]);
-                        to += __popc(m & below);
-                        found += __popc(m);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (hit[i]) rows[to++] = make_int2(r + i, __float_as_int(rest[r + i]));
-                    if (found <= SUM_LIST - SUM_EACH && b + 1 < b1) continue;
-                    __syncwarp();
-                    add_rows(a, rows, found, from, ldh);
-                    __syncwarp();
-                    found = 0;
-                }
-                s_part[warp][lane] = a;
-                __syncthreads();
-                if (tid < SUM_COLS && c0 + tid < d) {
-                    float s = 0.0f;
-                    for (int w = 0; w < SUM_WARPS; ++w) s += reinterpret_cast<const float*>(s_part[w])[tid];
-                    sums[to_row + c0 + tid] = s;
-                }
-                __syncthreads();
-            }
-        }
-        __syncthreads();
-    }
-}
 
 // Both products of a piece in one launch. kind 0: grad_hidden += G W (M rows, N
 // d_model, K the piece's columns, cut into `splits` where the tiles alone are
@@ -643,9 +524,11 @@ struct ProductOp {
     int split_width;          // the widest piece: what the number of splits goes by
     float* acc;               // sums of grad_hidden, a block of 256 x 256 per tile and split
     bool first, want_h, want_w;
-    const Group* groups;      // GradLogitsOp's
+    const int* counts;        // GradLogitsOp's
+    const Left* listed;
     const float* rest;
-    const float* sums;        // target_sums_kernel's, [group's row][lds]
+    const int* target;
+    float* sums;              // [first listed row][lds]: of a group's rests * hidden
     int lds;
     const T* h;               // the packed rows
     int ldh;
@@ -709,43 +592,187 @@ struct ProductOp {
         const int kr = t.kind >= 0 ? v0 + k : k;
         for (int j = 0; j < n / 128; ++j) mxs::gemm::tma_load<2>(sb + j * 8192, b, c + 64 * j, kr, bar);
     }
-    // What the target entries' roundings left out of this thread's vocabulary row, columns
-    // [c, c + 32): the one row's rest * hidden, or the sum over the rows that share it.
-    __device__ void add_rest(float (&v)[32], Group g, float left, int c) const {
-        if (g.count == 1) {
-            const T* row = h + (int64_t)g.row * ldh + c;
-            if (c + 32 <= ldh) {  // rows are whole 16-byte pieces; what lies past d is not stored
+    // What the rests of rows that share a target add to its grad_weight row, in ascending
+    // order of the rows whatever the order they were counted in. One row or two: the thread
+    // that holds the vocabulary row adds them (add_rest). More, for the CTA's 128 vocabulary
+    // rows and the tile's columns, before the tile's accumulator is waited for, under its
+    // products, whose time grows with the rows too: up to LISTED rows are sorted and summed
+    // by a warp, up to FEW found among all targets by a warp, more found and summed by all
+    // warps, each a sixteenth of the rows, and these sums added in order. Both gradients of
+    // 4096 x 32000 x 512: uniform targets 340 us, Zipf 405, 60 % on one id 392, all on one 360,
+    // on 32 neighbours 442.
+    static constexpr int FEW = 256;
+    static constexpr int EACH = 128, LIST = EACH + 32;  // targets looked at at once, and a warp's list
+
+    // a += rest * hidden of n listed rows, eight columns from `from` on, eight rows' loads in flight.
+    __device__ void add_rows(float (&a)[8], const int* list, int n, const T* from) const {
+        for (int e = 0; e < n; e += 8) {
+            uint4 u[8];
+            float f[8];
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(row + j);
-                    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) v[j + q] = fmaf(left, to_f32(e[q]), v[j + q]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j < d) v[j] = fmaf(left, to_f32(row[j]), v[j]);
+            for (int i = 0; i < 8; ++i) {
+                const int r = list[min(e + i, n - 1)];
+                f[i] = rest[r];
+                u[i] = *reinterpret_cast<const uint4*>(from + (int64_t)r * ldh);
             }
-        } else if (g.count > 1 && c < d) {  // lds is a multiple of 32
-            const float4* row = reinterpret_cast<const float4*>(sums + (int64_t)g.row * lds + c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float4 u = row[j];
-                v[4 * j] += u.x;
-                v[4 * j + 1] += u.y;
-                v[4 * j + 2] += u.z;
-                v[4 * j + 3] += u.w;
+            for (int i = 0; i < 8; ++i) {
+                if (e + i >= n) f[i] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[j] = fmaf(f[i], to_f32(reinterpret_cast<const T*>(&u[i])[j]), a[j]);
+            }
+        }
+    }
+    // The same for the rows with target v among blocks [b0, b1) of EACH rows.
+    __device__ void find_rows(float (&a)[8], int* list, int v, int b0, int b1, const T* from, int lane, int kept) const {
+        const int4* at = reinterpret_cast<const int4*>(target) + lane;
+        int found = 0;
+        __syncwarp();
+        int4 next = b0 < b1 ? at[(int64_t)b0 * (EACH / 4)] : make_int4(-1, -1, -1, -1);
+        for (int k = b0; k < b1; ++k) {
+            const int r = k * EACH + 4 * lane, here[4] = {next.x, next.y, next.z, next.w};
+            if (k + 1 < b1) next = at[(int64_t)(k + 1) * (EACH / 4)];
+            bool hit[4];
+            int to = found;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hit[j] = here[j] == v && r + j < kept;
+                const uint32_t w = __ballot_sync(0xffffffffu, hit[j]);
+                to += __popc(w & ((1u << lane) - 1));
+                found += __popc(w);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (hit[j]) list[to++] = r + j;
+            if (found <= LIST - EACH && k + 1 < b1) continue;
+            __syncwarp();
+            add_rows(a, list, found, from);
+            __syncwarp();
+            found = 0;
+        }
+    }
+    __device__ bool sum_groups(const Tile& t, int m, Lane& me, const Ctx& x) const {
+        constexpr int XPOSE = mxs::gemm::Geo<ProductOp>::XPOSE;
+        const int warp = me.grp * 4 + me.quad, c = t.n0 + me.lane * 8;
+        const bool mine = me.lane * 8 < n && c < ldh;  // rows are whole 16-byte pieces
+        const T* from = h + (mine ? c : 0);
+        float* part = reinterpret_cast<float*>(me.xpose);  // 256 columns' sums of this warp
+        int* list = reinterpret_cast<int*>(me.xpose + 1024);
+        const int blocks = (x.kept + EACH - 1) / EACH, per = (blocks + EPI - 1) / EPI;
+        int turn = 0;
+        for (int q = 0; q < 4; ++q) {
+            const int row = m + q * 32 + me.lane, count = row < width ? counts[v0 + row] : 0;
+            for (uint32_t b = __ballot_sync(0xffffffffu, count > 2 && count <= FEW); b; b &= b - 1) {
+                if (turn++ % EPI != warp) continue;
+                const int i = __ffs(b) - 1, n_rows = __shfl_sync(0xffffffffu, count, i), v = m + q * 32 + i;
+                const Left* of = listed + (int64_t)v * LISTED;
+                float a[8] = {};
+                if (n_rows <= LISTED) {
+                    const int r = me.lane < n_rows ? of[me.lane].row : INT_MAX;
+                    int to = 0;
+#pragma unroll
+                    for (int k = 0; k < LISTED; ++k) to += __shfl_sync(0xffffffffu, r, k) < r;
+                    __syncwarp();
+                    if (me.lane < n_rows) list[to] = r;
+                    __syncwarp();
+                    add_rows(a, list, n_rows, from);
+                } else {
+                    find_rows(a, list, v0 + v, 0, blocks, from, me.lane, x.kept);
+                }
+                if (mine) {
+                    float4* to = reinterpret_cast<float4*>(sums + (int64_t)of[0].row * lds + c);
+                    to[0] = make_float4(a[0], a[1], a[2], a[3]);
+                    to[1] = make_float4(a[4], a[5], a[6], a[7]);
+                }
+            }
+        }
+        for (int q = 0; q < 4; ++q) {
+            const int row = m + q * 32 + me.lane, count = row < width ? counts[v0 + row] : 0;
+            for (uint32_t b = __ballot_sync(0xffffffffu, count > FEW); b; b &= b - 1) {
+                const int v = m + q * 32 + __ffs(b) - 1;
+                float a[8] = {};
+                find_rows(a, list, v0 + v, min(blocks, warp * per), min(blocks, (warp + 1) * per), from, me.lane, x.kept);
+                reinterpret_cast<float4*>(part)[me.lane * 2] = make_float4(a[0], a[1], a[2], a[3]);
+                reinterpret_cast<float4*>(part)[me.lane * 2 + 1] = make_float4(a[4], a[5], a[6], a[7]);
+                if (!mxs::gemm::gather(me, x)) return false;
+                const int col = warp * 32 + me.lane;
+                if (col < n && t.n0 + col < d) {
+                    const float* first = reinterpret_cast<const float*>(me.xpose - warp * XPOSE) + col;
+                    float s = 0.0f;
+                    for (int w = 0; w < EPI; ++w) s += first[w * (XPOSE / 4)];
+                    sums[(int64_t)listed[(int64_t)v * LISTED].row * lds + t.n0 + col] = s;
+                }
+                if (!mxs::gemm::gather(me, x)) return false;  // before the parts are written again
+            }
+        }
+        return mxs::gemm::gather(me, x);
+    }
+    // The group of this thread's vocabulary row: its size and its first two (as they are listed).
+    struct Ahead {
+        int count;
+        int4 left;
+        bool ok;
+    };
+    __device__ Ahead ahead(const Tile& t, Lane& me, const Ctx& x) const {
+        Ahead it{0, make_int4(0, 0, 0, 0), true};
+        if (t.kind >= 0) return it;
+        const int m = t.m0 + (int)x.rank * 128;
+        bool many = false;  // a group to be summed among the CTA's
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = m + q * 32 + me.lane, count = row < width ? counts[v0 + row] : 0;
+            if (q == me.quad) it.count = count;
+            many |= count > 2;
+        }
+        if (m + me.row % 128 < width)
+            it.left = *reinterpret_cast<const int4*>(listed + (int64_t)(t.m0 + me.row) * LISTED);
+        if (__any_sync(0xffffffffu, many)) it.ok = sum_groups(t, m, me, x);
+        return it;
+    }
+    // v += rest * hidden of a row, columns [c, c + 32).
+    __device__ void add_row(float (&v)[32], int r, float left, int c) const {
+        const T* row = h + (int64_t)r * ldh + c;
+        if (c + 32 <= ldh) {  // rows are whole 16-byte pieces; what lies past d is not stored
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+                const uint4 u = *reinterpret_cast<const uint4*>(row + j);
+                const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[j + q] = fmaf(left, to_f32(e[q]), v[j + q]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (c + j < d) v[j] = fmaf(left, to_f32(row[j]), v[j]);
+        }
+    }
+    // What the target entries' roundings left out of this thread's vocabulary row, columns [c, c + 32).
+    __device__ void add_rest(float (&v)[32], const Ahead& it, int c) const {
+        if (it.count > 2) {
+            if (c < d) {  // lds is a multiple of 32
+                const float4* row = reinterpret_cast<const float4*>(sums + (int64_t)it.left.x * lds + c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float4 u = row[j];
+                    v[4 * j] += u.x;
+                    v[4 * j + 1] += u.y;
+                    v[4 * j + 2] += u.z;
+                    v[4 * j + 3] += u.w;
+                }
+            }
+        } else {
+            const bool swap = it.count == 2 && it.left.z < it.left.x;
+            for (int k = 0; k < it.count; ++k) {
+                const bool second = (k == 1) != swap;
+                add_row(v, second ? it.left.z : it.left.x, __int_as_float(second ? it.left.w : it.left.y), c);
             }
         }
         __syncwarp();
     }
-    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&) const {
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, const Ahead& it) const {
         // two factors: their product may leave fp32's range where the results do not
         const float gmax = t.kind >= 0 ? 1.0f : head->gmax;
         const int m = t.m0 + me.row - me.lane;  // first row of the warp
-        const Group group = t.kind < 0 && m + me.lane < width ? groups[v0 + m + me.lane] : Group{0, 0};
-        const float left = group.count == 1 ? rest[group.row] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c0 = me.grp * 32 + i * 128;
@@ -759,7 +786,7 @@ struct ProductOp {
                 else
                     mxs::gemm::store_rows<float, true>(a, 256, v, 32, 32, true, me);
             } else {
-                add_rest(v, group, left, t.n0 + c0);
+                add_rest(v, it, t.n0 + c0);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = v[j] * scale * gmax;
                 mxs::gemm::store_rows<T, false>(dw + (int64_t)(v0 + m) * lddw + t.n0 + c0, lddw, v, width - m,
@@ -837,8 +864,8 @@ struct Plan {
     Head* head;
     void* packed;
     int *pos, *target;
-    Group* groups;
-    int* listed;
+    int* counts;
+    Left* listed;
     float *rest, *sums;
     float2* part;
     float *ytarget, *lse2, *ghat, *acc;
@@ -885,7 +912,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
     } else {
         pl.lse2 = c.take<float>(rows);
         pl.ghat = c.take<float>(rows);
-        pl.groups = c.take<Group>(vocab);
+        pl.counts = c.take<int>(vocab);
         pl.rest = c.take<float>(rows);
         pl.lds = (int)round_up(d, 32);
         pl.sums = c.take<float>((size_t)rows * pl.lds);
@@ -893,7 +920,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
         pl.piece = round_up(ceil_div(vocab, ceil_div(vocab, most)), 256);
         plan_tiles(pl, sms, rows, std::min(pl.piece, vocab));
         pl.g = c.take<uint16_t>((size_t)rp * pl.piece);
-        pl.listed = c.take<int>((size_t)pl.piece * LISTED);
+        pl.listed = c.take<Left>((size_t)pl.piece * LISTED);
         pl.dn = d > 128 ? 256 : 128;
         pl.dnt = (int)ceil_div(d, pl.dn);
         pl.acc = c.take<float>((size_t)std::max<int64_t>(rp / 256 * pl.dnt, sms / 2) * 65536);
@@ -948,8 +975,8 @@ struct Call {
 template <typename T>
 int pack_rows(const Call& a, const Plan& pl, const float* lse, const float* grad, bool want_w) {
     const Pack p{a.hidden, a.ldh, a.targets, (int)a.rows, (int)a.d, pl.ldk, lse, grad, pl.head,
-                 pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat, want_w ? pl.groups : nullptr};
-    // a CTA for four rows, and for 2048 groups to be emptied
+                 pl.packed, pl.pos, pl.target, pl.lse2, pl.ghat, want_w ? pl.counts : nullptr};
+    // a CTA for four rows, and for 2048 counts to be zeroed
     const int64_t ctas = std::max(ceil_div(a.rows, 4), want_w ? ceil_div(a.vocab, 8 * PACK_T) : 0);
     MXS_TRY(launch_dependent(pack_rows_kernel<T>, (unsigned)std::min<int64_t>(ctas, a.sms * 4), PACK_T, a.st, p));
     return MXS_OK;
@@ -1010,7 +1037,7 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     op.ghat = pl.ghat;
     op.g = static_cast<T*>(pl.g);
     op.rest = pl.rest;
-    op.groups = prod.want_w ? pl.groups : nullptr;
+    op.counts = prod.want_w ? pl.counts : nullptr;
     op.listed = pl.listed;
     op.ldg = (int)pl.piece;
     // f16 holds G times 2^14: the target's entry stays below its largest value
@@ -1018,13 +1045,6 @@ int grad_piece(const Call& a, const Plan& pl, const void* w, int64_t ldw, int64_
     op.gscale = format_of<T>() == 0 ? 16384.0f : 1.0f;
     const int64_t units = CG == 1 ? ceil_div(op.vocab, pl.span) : ceil_div(a.rows, 256) * op.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
-    if (prod.want_w) {
-        const int64_t chunks = std::min<int64_t>(ceil_div(a.d, SUM_COLS), 65535);
-        const int64_t each = std::min<int64_t>(op.vocab, std::max<int64_t>(1, 2 * a.sms / chunks));
-        MXS_TRY(launch_dependent(target_sums_kernel<T>, dim3((unsigned)each, (unsigned)chunks), SUM_WARPS * 32, a.st,
-                                 pl.head, pl.groups, pl.listed, (int)v0, op.vocab, pl.target, pl.rest,
-                                 static_cast<const T*>(pl.packed), pl.ldk, (int)a.d, pl.sums, pl.lds));
-    }
     prod.v0 = (int)v0;
     prod.width = op.vocab;
     prod.first = v0 == 0;
@@ -1073,9 +1093,11 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
     prod.nt = pl.dnt;
     prod.split_width = (int)std::min(pl.piece, a.vocab);
     prod.acc = pl.acc;
-    prod.groups = pl.groups;
+    prod.counts = pl.counts;
     prod.rest = pl.rest;
     prod.sums = pl.sums;
+    prod.listed = pl.listed;
+    prod.target = pl.target;
     prod.lds = pl.lds;
     prod.h = static_cast<const T*>(pl.packed);
     prod.ldh = pl.ldk;

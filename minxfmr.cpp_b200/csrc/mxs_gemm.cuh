@@ -69,12 +69,12 @@ struct Lane {
     int lane, quad, grp;  // quad: which 32 rows of the CTA's 128; grp: which column group
     int row;              // of the pair's tile
     uint8_t* xpose;       // its warp's bytes for transposes
-    int meetings;         // how often the warps of this quad have met
+    int meetings, gatherings;  // how often the warps of this quad, and all of the CTA's, have met
 };
 
 struct Ring {
     uint64_t full[6], empty[6], tfull[MAX_ACC], tempty[MAX_ACC], drain;
-    uint64_t meet[4];  // of each quad's warps, where an Op has them meet
+    uint64_t meet[5];  // of each quad's warps, and of all epilogue warps, where an Op has them meet
     uint32_t tmem;
     int dead;
 };
@@ -319,13 +319,18 @@ struct Ctx {
     Ring* ring;
 };
 
-// The warps of a quad meet: what each wrote to shared memory before is there for all
-// after. False when one of them has given up.
-__device__ __forceinline__ bool meet(Lane& me, const Ctx& x) {
-    uint64_t* bar = &x.ring->meet[me.quad];
+// Warps meet: what each wrote to memory before is there for all after. False when one of
+// them has given up.
+__device__ __forceinline__ bool meet_at(uint64_t* bar, int& times, const Lane& me, const Ctx& x) {
     __syncwarp();
     if (me.lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-    return __all_sync(0xffffffffu, wait(bar, me.meetings++ & 1, x.ring));
+    return __all_sync(0xffffffffu, wait(bar, times++ & 1, x.ring));
+}
+__device__ __forceinline__ bool meet(Lane& me, const Ctx& x) {  // of a quad
+    return meet_at(&x.ring->meet[me.quad], me.meetings, me, x);
+}
+__device__ __forceinline__ bool gather(Lane& me, const Ctx& x) {  // all epilogue warps of the CTA
+    return meet_at(&x.ring->meet[4], me.gatherings, me, x);
 }
 
 // The kernel body. Op (a __grid_constant__ parameter) has
@@ -346,7 +351,8 @@ __device__ __forceinline__ bool meet(Lane& me, const Ctx& x) {
 //   bytes(t)               bytes this CTA loads per block
 //   load(t, kb, sa, sb, bar, ctx)
 //   zero(t, me, ctx)                                    the epilogue of a tile without blocks
-//   epilogue(t, tmem, me, ctx)                          !PROMOTE
+//   ahead(t, me, ctx), epilogue(t, tmem, me, ctx, it)   !PROMOTE: `it` is what ahead gave, before the
+//                          accumulator was waited for; it.ok is false where its warps did not meet
 //   group(), Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulator is
 //                          read back and joined in registers after each `group` blocks; finish
 //                          says false where its warps did not meet
@@ -375,7 +381,7 @@ __device__ __forceinline__ void run(const Op& op) {
             mbar_init(&ring->tempty[i], Op::EPI * CG);
         }
         mbar_init(&ring->drain, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(&ring->meet[i], Op::EPI / 4);
+        for (int i = 0; i < 5; ++i) mbar_init(&ring->meet[i], i < 4 ? Op::EPI / 4 : Op::EPI);
         ring->dead = 0;
         fence_mbar_init();
         op.prefetch();
@@ -499,7 +505,7 @@ __device__ __forceinline__ void run(const Op& op) {
         me.grp = (warp - EPI_WARP0) >> 2;
         me.row = (int)ctx.rank * 128 + me.quad * 32 + lane;
         me.xpose = xpose + (warp - EPI_WARP0) * G::XPOSE;
-        me.meetings = 0;
+        me.meetings = me.gatherings = 0;
         const uint32_t lanes = (uint32_t)(me.quad * 32) << 16;
         const bool remote = CG == 2 && ctx.rank != 0;
         const uint32_t te0 = remote ? map_to_rank(smem_u32(&ring->tempty[0]), 0) : smem_u32(&ring->tempty[0]);
@@ -529,10 +535,11 @@ __device__ __forceinline__ void run(const Op& op) {
                 }
                 if (ok) ok = op.finish(acc, t, me, ctx);
             } else {
-                ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
+                const auto it = op.ahead(t, me, ctx);
+                ok = it.ok && __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
                 if (!ok) break;
                 fence_after();
-                op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx);
+                op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx, it);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive(te0 + buf * 8, remote);

@@ -105,13 +105,17 @@ def repeated(kind, rows, vocab, g):
         sizes = torch.tensor([1, 2, 3, 15, 16, 17, 18, 33] * (rows // 105 + 1), device="cuda")
         t = (torch.arange(len(sizes), device="cuda") * 5 % vocab).repeat_interleave(sizes)[:rows]
         t = t[torch.randperm(rows, generator=g, device="cuda")]
+    elif kind == "large":  # and on either side of 256
+        sizes = torch.tensor([256, 1, 257, 2, 300, 5, 255, 40] * (rows // 1116 + 1), device="cuda")
+        t = (torch.arange(len(sizes), device="cuda") * 3 % vocab).repeat_interleave(sizes)[:rows]
+        t = t[torch.randperm(rows, generator=g, device="cuda")]
     elif kind == "runs":  # each target's rows side by side
         t = torch.arange(rows, device="cuda") * 7 // max(rows, 7) * (vocab // 7)
     return t
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
-@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts"])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts", "large"])
 @pytest.mark.parametrize("rows,vocab,d", [(2, 300, 9), (130, 1000, 200), (700, 513, 264), (2500, 4001, 72)])
 def test_repeated_targets(mxs, rows, vocab, d, kind, dt):
     g = gen(rows + vocab)
@@ -126,8 +130,8 @@ def test_repeated_targets(mxs, rows, vocab, d, kind, dt):
 
 
 @pytest.mark.parametrize("dt,vocab", [(BF, 512), (HF, 4096)])
-@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts", "uniform"])
-@pytest.mark.parametrize("rows,d", [(90, 33), (1000, 300)])
+@pytest.mark.parametrize("kind", ["one", "most", "neighbours", "zipf", "runs", "counts", "large", "uniform"])
+@pytest.mark.parametrize("rows,d", [(90, 33), (1000, 300), (3000, 100)])
 def test_target_entries_keep_32_bits(mxs, rows, d, kind, dt, vocab):
     """A weight of zeros makes every probability 1 / vocab, a power of two, which the
     type holds, and every target entry 1 / vocab - 1, which it does not: the weight's
