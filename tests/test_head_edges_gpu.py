@@ -89,6 +89,33 @@ def test_warps_that_meet_give_up(mxs, rows, tile):
     assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
 
 
+@pytest.mark.parametrize("tile", [0, 1])
+def test_warps_that_gather_give_up(mxs, tile):
+    """The same for the warps of a CTA that sum a target's rows together in the gradient
+    product: the one that leaves does so before a tile whose vocabulary rows have such a
+    target."""
+    rows, vocab, d = 600, 40000, 64
+    h, w, _ = operands(rows, vocab, d, BF, seed=41)
+    t = torch.where(torch.arange(rows, device="cuda") % 2 == 0, 5, 74 * 256 + 5)  # CTA 0's first and second tile
+    grad = torch.ones(rows, device="cuda")
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    def call():
+        out = mxs.ce_from_hidden_backward(h, w, t, lse, grad, need_hidden=False)[1]
+        torch.cuda.synchronize()
+        return out
+    before = call()
+    mxs.get_status(clear=True)
+    mxs.set_test_hooks(drop_tile=-2 - tile)
+    try:
+        call()
+    finally:
+        mxs.set_test_hooks()
+    assert mxs.get_status(clear=True) & mxs.ROW_TIMEOUT
+    after = call()
+    assert mxs.get_status(clear=True) == 0
+    assert torch.equal(before, after)
+
+
 def repeated(kind, rows, vocab, g):
     """Targets as tokens have them: some far more often than others."""
     t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
