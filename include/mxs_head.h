@@ -43,8 +43,9 @@ extern "C" {
  *   d_hidden  rows x d_model of `dtype` (MXS_BF16 or MXS_F16), row r at d_hidden + r*ld_hidden elements
  *   d_weight  vocab x d_model of `dtype`, row v at d_weight + v*ld_weight elements
  *   d_targets rows integers of target_bytes (4 or 8) bytes. A row whose target is
- *             outside [0, vocab) is left out: loss and lse are 0, its hidden state
- *             is not read (it may hold NaN), and it costs no products.
+ *             outside [0, vocab) is left out: loss and lse are 0, and its hidden
+ *             state (it may hold NaN) reaches no output. Above 128 rows it is not
+ *             read either and costs no products.
  *   d_loss, d_lse  rows floats; either may be NULL
  * Products are exact in fp32 and accumulated in fp32; maxima and sums of the
  * softmax are fp32. Limits: vocab, rows, d_model < 2^31 - 1024; temperature > 0.
@@ -101,7 +102,8 @@ MXS_API int mxs_quantize_fp8(const void* d_x, int64_t ld_x, int dtype, int64_t r
  * the product of a rows x k and an n x k matrix of 8-bit floats with a scale
  * for each 1 x 128 block of a and each 128 x 128 block of b, as
  * mxs_quantize_fp8 makes them. Each block of 128 products is summed in fp32 and
- * joined under its scales in fp32; out (MXS_F32, MXS_BF16 or MXS_F16; leading
+ * joined under its scales in fp32, whose product is formed first (it keeps its 24
+ * bits between 2^-126 and 2^128); out (MXS_F32, MXS_BF16 or MXS_F16; leading
  * dimension ld_out) is rounded once. Limits: rows, n, k < 2^31 - 1024.
  */
 MXS_API int mxs_matmul_fp8(const void* d_a, int64_t ld_a, const float* d_a_scale, const void* d_b, int64_t ld_b,

@@ -254,8 +254,10 @@ cudaError_t launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
 // The product. A stage of the ring is one block of 128 of K (128 bytes of a
 // row), so the accumulator of one block is one group: it is read back, scaled
 // by a_scale * b_scale and added in registers while the MMAs of the next block
-// fill the other accumulator (512 clocks of MMA for a 128 x 256 block, against
-// 256 of accumulator reads and 256 of FMA a scheduler).
+// fill the other accumulator. That join bounds the product above 128 rows: a block
+// takes 930 clocks where its MMAs take 512. Its reads (256 clocks) and its FMAs (256
+// a scheduler) would fit below them, but a warp waits for each 32 columns it reads
+// before it adds them, and there are two warps a scheduler to fill the gaps.
 // ---------------------------------------------------------------------------
 
 // The i-th tile of a CTA that walks its own `span` of the columns, n at a time, so

@@ -10,7 +10,8 @@
 // Warps 0..3 give up registers for the epilogue's (setmaxnreg). With 16 epilogue
 // warps: 640 threads x 96 at launch = 128 x 64 + 512 x 104; with 8: 384 x 168 =
 // 128 x 56 + 256 x 224. Sixteen suit epilogues with many instructions, eight the
-// 8-bit product, which keeps 128 sums a thread and loads in flight beside them.
+// 8-bit product, which keeps 128 sums a thread beside the 32 values it has just read
+// (a read of the accumulator is waited for before the next one is issued).
 //
 // A tile is 128 rows per CTA by up to 256 columns. With CG = 2 a pair of CTAs
 // works on one 256-row tile: each loads its 128 rows of A and half of B's
