@@ -4,7 +4,10 @@ product, and sampling from an 8-bit head.
 
 As in the rest of the package torch only carries memory and streams. Outputs and
 scratch are torch tensors of the call's stream (`stream`, or the current one), so
-calls on different streams share none.
+calls on different streams share none. Inputs are the caller's, as with torch's
+operations under torch.cuda.stream: the call does not wait for the stream they were
+made on, and a tensor given to another stream than its own is kept (or recorded
+there) until that stream has used it.
 """
 import contextlib
 import ctypes

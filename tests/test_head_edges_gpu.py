@@ -245,6 +245,25 @@ def test_gradients_in_several_pieces(mxs, rows, vocab, d, pieces, dt):
     check_ce(mxs, *in_pieces(mxs, rows, vocab, d, dt, rows + d, pieces), 0.9)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("rows,vocab,d", [(4000, 70001, 72), (4000, 40001, 300)])
+def test_repeated_targets_at_the_edges_of_pieces(mxs, rows, vocab, d, dt):
+    """Groups of every kind (2, 3, 16, 17, 256, 257 rows and more) on both sides of an edge
+    and in the vocabulary's last rows; again with the same bits."""
+    piece = piece_of(rows, vocab)
+    h, w, t = in_pieces(mxs, rows, vocab, d, dt, 7, ceil_div(vocab, piece))
+    at = 100
+    for target, count in ((piece - 1, 700), (piece, 257), (piece + 1, 17), (piece - 2, 3), (vocab - 1, 256),
+                          (vocab - 2, 300), (vocab - 3, 16), (0, 400), (piece - 128, 40), (piece - 129, 5)):
+        t[at:at + count] = target
+        at += count
+    t = t[torch.randperm(rows, generator=gen(2), device="cuda")]
+    grad = torch.randn(rows, generator=gen(9), device="cuda")
+    _, lse, gh, gw = check_ce(mxs, h, w, t, 0.9, grad)
+    again = mxs.ce_from_hidden_backward(h, w, t, lse, grad, temperature=0.9)
+    assert torch.equal(again[0], gh) and torch.equal(again[1], gw)
+
+
 def hidden_splits(rows, nt, width, units):
     """Splits of K for grad_hidden alone (grad_hidden_splits in mxs_ce.cu)."""
     tiles, blocks = ceil_div(rows, 256) * nt, ceil_div(width, 64)
