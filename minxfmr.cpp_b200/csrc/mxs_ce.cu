@@ -45,9 +45,9 @@ using mxs::gemm::Lane;
 using mxs::gemm::Tile;
 
 constexpr int64_t MAX_DIM = INT32_MAX - 1024;
-// What a wait of at most a second spans grows with the rows: grad_weight's run of products
-// (512 clocks at least for each 64 rows) and, where more than 16 rows share a target, the
-// looking for them (128 such targets a CTA). 2^24 rows take half of it at most.
+// What a wait of at most a second spans grows with the rows where more than 16 of them share
+// a target: a CTA's warps look for the rows of up to 128 such targets. 2^24 rows of 128 targets
+// take 0.4 s.
 constexpr int64_t MAX_BACKWARD_ROWS = 1 << 24;
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.4426950408889634074;
@@ -467,7 +467,7 @@ struct GradLogitsOp : LogitTiles<CG_> {
         static constexpr bool ok = true;
     };
     __device__ Ahead ahead(const Tile&, const Lane&, const Ctx&) const { return {}; }
-    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x, Ahead) const {
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx& x, Ahead, int) const {
         const int r = t.m0 + me.row;
         const bool live = r < x.kept;
         const int hit = live ? this->target[r] - this->v0 - t.n0 : -1;
@@ -508,16 +508,20 @@ struct GradLogitsOp : LogitTiles<CG_> {
     }
 };
 
-// Both products of a piece in one launch. kind 0: grad_hidden += G W (M rows, N
+// Both products of a piece in one launch. kind >= 0: grad_hidden += G W (M rows, N
 // d_model, K the piece's columns, cut into `splits` where the tiles alone are
-// fewer than the pairs); kind 1: grad_weight = G^T H (M the piece's columns, N
+// fewer than the pairs); kind < 0: grad_weight = G^T H (M the piece's columns, N
 // d_model, K rows). G is read K-major for the first and M-major for the second.
 template <typename T>
 struct ProductOp {
     static constexpr int CG = 2;
     static constexpr int EPI = 16, SWAP = 0;
     static constexpr bool F8 = false, PROMOTE = false;
-    __device__ int group() const { return INT32_MAX; }
+    // Sums of more than 32768 products are added up in fp32 after so many: the MMA's own
+    // sum rounds towards zero at every 16 of them, which by then may have cost 2^-13 of it
+    // (2 million rows of one sign, in one run: 8 parts in a thousand).
+    static constexpr int RUN = 512;
+    __device__ int group() const { return RUN; }
     CUtensorMap g_k, g_m, w_n, h_n;
     int format;
     int64_t drop;
@@ -526,6 +530,7 @@ struct ProductOp {
     int v0, width, d, n, nt;  // nt tiles of n columns over d
     int split_width;          // the widest piece: what the number of splits goes by
     float* acc;               // sums of grad_hidden, a block of 256 x 256 per tile and split
+    float* runs;              // [CTA][128][256]: sums of grad_weight so far, where they take several runs
     bool first, want_h, want_w;
     const int* counts;        // GradLogitsOp's
     const Left* listed;
@@ -627,7 +632,8 @@ struct ProductOp {
         }
     }
     // The same for the rows with target v among blocks [b0, b1) of EACH rows.
-    __device__ void find_rows(float (&a)[8], int* list, int v, int b0, int b1, const T* from, int lane, int kept) const {
+    __device__ void find_rows(float (&a)[8], int* list, int v, int b0, int b1, const T* from, int lane,
+                              int kept) const {
         const int4* at = reinterpret_cast<const int4*>(target) + lane;
         int found = 0;
         __syncwarp();
@@ -694,7 +700,8 @@ struct ProductOp {
             for (uint32_t b = __ballot_sync(0xffffffffu, count > FEW); b; b &= b - 1) {
                 const int v = m + q * 32 + __ffs(b) - 1;
                 float a[8] = {};
-                find_rows(a, list, v0 + v, min(blocks, warp * per), min(blocks, (warp + 1) * per), from, me.lane, x.kept);
+                const int b0 = min(blocks, warp * per), b1 = min(blocks, b0 + per);
+                find_rows(a, list, v0 + v, b0, b1, from, me.lane, x.kept);
                 reinterpret_cast<float4*>(part)[me.lane * 2] = make_float4(a[0], a[1], a[2], a[3]);
                 reinterpret_cast<float4*>(part)[me.lane * 2 + 1] = make_float4(a[4], a[5], a[6], a[7]);
                 if (!mxs::gemm::gather(me, x)) return false;
@@ -772,7 +779,8 @@ struct ProductOp {
         }
         __syncwarp();
     }
-    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, const Ahead& it) const {
+    __device__ void epilogue(const Tile& t, uint32_t tmem, const Lane& me, const Ctx&, const Ahead& it, int kb) const {
+        const bool last = kb + RUN >= t.kn;
         // two factors: their product may leave fp32's range where the results do not
         const float gmax = t.kind >= 0 ? 1.0f : head->gmax;
         const int m = t.m0 + me.row - me.lane;  // first row of the warp
@@ -784,11 +792,27 @@ struct ProductOp {
             mxs::gemm::tmem_ld32(tmem + c0, v);
             if (t.kind >= 0) {
                 float* a = acc + ((int64_t)t.kind * 256 + me.row - me.lane) * 256 + c0;
-                if (first)
+                if (first && kb == 0)
                     mxs::gemm::store_rows<float, false>(a, 256, v, 32, 32, true, me);
                 else
                     mxs::gemm::store_rows<float, true>(a, 256, v, 32, 32, true, me);
             } else {
+                if (!last || kb > 0) {
+                    float* a = runs + ((int64_t)blockIdx.x * 128 + me.quad * 32) * 256 + c0;
+                    if (kb == 0)
+                        mxs::gemm::store_rows<float, false>(a, 256, v, 32, 32, true, me);
+                    else
+                        mxs::gemm::store_rows<float, true>(a, 256, v, 32, 32, true, me);
+                    if (!last) continue;
+                    __syncwarp();
+                    const float4* sum = reinterpret_cast<const float4*>(a + me.lane * 256);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 u = sum[j];
+                        v[4 * j] = u.x, v[4 * j + 1] = u.y, v[4 * j + 2] = u.z, v[4 * j + 3] = u.w;
+                    }
+                    __syncwarp();
+                }
                 add_rest(v, it, t.n0 + c0);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = v[j] * scale * gmax;
@@ -869,7 +893,7 @@ struct Plan {
     int *pos, *target;
     int* counts;
     Left* listed;
-    float *rest, *sums;
+    float *rest, *sums, *runs;
     float2* part;
     float *ytarget, *lse2, *ghat, *acc;
     void* g;
@@ -926,6 +950,7 @@ Plan make_plan(void* ws, int sms, const void* weight, int64_t ldw, int64_t rows,
         pl.listed = c.take<Left>((size_t)pl.piece * LISTED);
         pl.dn = d > 128 ? 256 : 128;
         pl.dnt = (int)ceil_div(d, pl.dn);
+        if (rows > 64 * ProductOp<__half>::RUN) pl.runs = c.take<float>((size_t)sms * 128 * 256);
         pl.acc = c.take<float>((size_t)std::max<int64_t>(rp / 256 * pl.dnt, sms / 2) * 65536);
     }
     pl.bytes = c.used;
@@ -1099,6 +1124,7 @@ int backward(const Call& a, const Plan& pl, const float* lse, const float* grad,
     prod.counts = pl.counts;
     prod.rest = pl.rest;
     prod.sums = pl.sums;
+    prod.runs = pl.runs;
     prod.listed = pl.listed;
     prod.target = pl.target;
     prod.lds = pl.lds;

@@ -352,11 +352,12 @@ __device__ __forceinline__ bool gather(Lane& me, const Ctx& x) {  // all epilogu
 //   bytes(t)               bytes this CTA loads per block
 //   load(t, kb, sa, sb, bar, ctx)
 //   zero(t, me, ctx)                                    the epilogue of a tile without blocks
-//   ahead(t, me, ctx), epilogue(t, tmem, me, ctx, it)   !PROMOTE: `it` is what ahead gave, before the
-//                          accumulator was waited for; it.ok is false where its warps did not meet
-//   group(), Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulator is
-//                          read back and joined in registers after each `group` blocks; finish
-//                          says false where its warps did not meet
+//   group()                blocks after which an accumulator is read back
+//   ahead(t, me, ctx), epilogue(t, tmem, me, ctx, it, kb)  !PROMOTE: kb, the first block of what the
+//                          accumulator holds; `it` is what ahead gave, before the tile's first was
+//                          waited for; it.ok is false where its warps did not meet
+//   Acc, begin(...), prepare(...), join(...), finish(...)  PROMOTE: the accumulators of a tile are
+//                          joined in registers; finish says false where its warps did not meet
 template <typename Op>
 __device__ __forceinline__ void run(const Op& op) {
     constexpr int CG = Op::CG;
@@ -537,14 +538,17 @@ __device__ __forceinline__ void run(const Op& op) {
                 if (ok) ok = op.finish(acc, t, me, ctx);
             } else {
                 const auto it = op.ahead(t, me, ctx);
-                ok = it.ok && __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
-                if (!ok) break;
-                fence_after();
-                op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx, it);
-                fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(te0 + buf * 8, remote);
-                if (++buf == accs) buf = 0, tph ^= 1;
+                ok = it.ok;
+                for (int kb = 0; ok && kb < t.kn; kb += min(op.group(), t.kn)) {
+                    ok = __all_sync(0xffffffffu, wait(&ring->tfull[buf], tph, ring));
+                    if (!ok) break;
+                    fence_after();
+                    op.epilogue(t, tmem + buf * acc_cols + lanes, me, ctx, it, kb);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(te0 + buf * 8, remote);
+                    if (++buf == accs) buf = 0, tph ^= 1;
+                }
             }
         }
     }

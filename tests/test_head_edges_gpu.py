@@ -478,3 +478,42 @@ def test_f16_gradient_weights_of_many_sizes(mxs):
         b = mxs.ce_from_hidden_backward(h, w, t, lse, grad * scale)[0]
         ok = (a.abs() >= 2.0 ** -2) & (b.abs() >= 2.0 ** -13)  # both in f16's normal range
         assert ok.any() and torch.equal((a.double() * scale)[ok], b.double()[ok])
+
+
+@pytest.mark.parametrize("rows,dt,vocab,kind", [(200000, BF, 512, "one"), (200000, HF, 4096, "uniform"),
+                                                (1000000, BF, 512, "uniform"), (1000000, HF, 512, "one"),
+                                                (33000, HF, 4096, "one"), (65536, HF, 4096, "one")])
+def test_weight_gradient_of_many_rows(mxs, rows, dt, vocab, kind):
+    """Sums over the rows in which all terms have one sign (a weight of zeros makes every
+    probability 1 / vocab). The MMA's own fp32 sum loses up to 2^-23 of itself at every
+    16 products, 2^-13 of the whole over 32768 of them; joined after so many, the
+    total loses no more than that, and the result's rounding."""
+    g = gen(rows + vocab)
+    h = (torch.rand((rows, 16), generator=g, device="cuda") + 0.5).to(dt)
+    w = torch.zeros((vocab, 16), dtype=dt, device="cuda")
+    t = repeated(kind, rows, vocab, g)
+    grad = torch.full((rows,), 2.0 ** -10, device="cuda")  # f16 results stay in range
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    gh, gw = mxs.ce_from_hidden_backward(h, w, t, lse, grad)
+    p = h.double().sum(0) / vocab * 2.0 ** -10
+    hot = torch.zeros((vocab, 16), dtype=torch.float64, device="cuda").index_add_(0, t, h.double() * 2.0 ** -10)
+    want = p - hot
+    assert ((gw.double() - want).abs() <= head_ref.U[dt] * want.abs() + 2.0 ** -13 * (p + hot) + 2.0 ** -25).all()
+    assert (gh == 0).all()
+
+
+def test_hidden_gradient_of_a_long_vocabulary(mxs):
+    """The same for sums over a piece of 32768 columns and more: 2500 rows whose weight
+    rows are all alike, 40000 columns in one piece."""
+    rows, vocab, d = 2500, 40000, 16
+    assert piece_of(rows, vocab) > 32768
+    g = gen(3)
+    w = (torch.rand((1, d), generator=g, device="cuda") + 0.5).to(HF).repeat(vocab, 1)
+    h = torch.zeros((rows, d), dtype=HF, device="cuda")
+    w[7] = 0
+    t = torch.full((rows,), 7, device="cuda")
+    _, lse = mxs.ce_from_hidden(h, w, t)
+    gh, _ = mxs.ce_from_hidden_backward(h, w, t, lse, torch.ones(rows, device="cuda"), need_weight=False)
+    want = w.double().sum(0) / vocab  # the target's own row is zero
+    # the probabilities' rounding to f16 is common to all columns: 2^-11 of the sum, and the result's
+    assert ((gh.double() - want).abs() <= (2 * 2.0 ** -11 + 2.0 ** -13) * want).all()
