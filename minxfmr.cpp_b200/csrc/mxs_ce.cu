@@ -607,8 +607,8 @@ struct ProductOp {
     // products, whose time grows with the rows too: up to LISTED rows are sorted and summed
     // by a warp, up to FEW found among all targets by a warp, more found and summed by all
     // warps, each a sixteenth of the rows, and these sums added in order. Both gradients of
-    // 4096 x 32000 x 512: uniform targets 340 us, Zipf 405, 60 % on one id 392, all on one 360,
-    // on 32 neighbours 442.
+    // 4096 x 32000 x 512: uniform targets 348 us, Zipf 408, 60 % on one id 396, all on one 374,
+    // on 32 neighbours 416.
     static constexpr int FEW = 256;
     static constexpr int EACH = 128, LIST = EACH + 32;  // targets looked at at once, and a warp's list
 
@@ -637,28 +637,37 @@ struct ProductOp {
         const int4* at = reinterpret_cast<const int4*>(target) + lane;
         int found = 0;
         __syncwarp();
-        int4 next = b0 < b1 ? at[(int64_t)b0 * (EACH / 4)] : make_int4(-1, -1, -1, -1);
-        for (int k = b0; k < b1; ++k) {
-            const int r = k * EACH + 4 * lane, here[4] = {next.x, next.y, next.z, next.w};
-            if (k + 1 < b1) next = at[(int64_t)(k + 1) * (EACH / 4)];
-            bool hit[4];
-            int to = found;
+        for (int k0 = b0; k0 < b1; k0 += 4) {  // four blocks' loads in flight
+            int4 u[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                hit[j] = here[j] == v && r + j < kept;
-                const uint32_t w = __ballot_sync(0xffffffffu, hit[j]);
-                to += __popc(w & ((1u << lane) - 1));
-                found += __popc(w);
+            for (int i = 0; i < 4; ++i) u[i] = at[(int64_t)min(k0 + i, b1 - 1) * (EACH / 4)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = (k0 + i) * EACH + 4 * lane, here[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                bool hit[4], any = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) any |= hit[j] = here[j] == v && r + j < kept && k0 + i < b1;
+                if (!__any_sync(0xffffffffu, any)) continue;
+                int to = found;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = __ballot_sync(0xffffffffu, hit[j]);
+                    to += __popc(w & ((1u << lane) - 1));
+                    found += __popc(w);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (hit[j]) list[to++] = r + j;
+                if (found <= LIST - EACH) continue;
+                __syncwarp();
+                add_rows(a, list, found, from);
+                __syncwarp();
+                found = 0;
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (hit[j]) list[to++] = r + j;
-            if (found <= LIST - EACH && k + 1 < b1) continue;
-            __syncwarp();
-            add_rows(a, list, found, from);
-            __syncwarp();
-            found = 0;
         }
+        __syncwarp();
+        add_rows(a, list, found, from);
+        __syncwarp();
     }
     __device__ bool sum_groups(const Tile& t, int m, Lane& me, const Ctx& x) const {
         constexpr int XPOSE = mxs::gemm::Geo<ProductOp>::XPOSE;
