@@ -47,8 +47,9 @@ extern "C" {
  *             state (it may hold NaN) reaches no output. Above 128 rows it is not
  *             read either and costs no products.
  *   d_loss, d_lse  rows floats; either may be NULL
- * Products are exact in fp32 and accumulated in fp32; maxima and sums of the
- * softmax are fp32. Limits: vocab, rows, d_model < 2^31 - 1024; temperature > 0.
+ * Products are accumulated in fp32, rounded towards zero within runs of 256 (up to
+ * 128 rows) or 512 and to nearest between them; maxima and sums of the softmax are
+ * fp32. Limits: vocab, rows, d_model < 2^31 - 1024; temperature > 0.
  */
 MXS_API int mxs_ce_from_hidden(const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
                                int dtype, int64_t rows, int64_t d_model, int64_t vocab, const void* d_targets,

@@ -296,13 +296,18 @@ struct LogitTiles {
 // clocks of MMA for each 64 of d_model.
 // The MMA's own fp32 sum rounds towards zero at every 16 products, which at
 // d_model 3584 leaves 2e-6 of the logits' size; the accumulator is joined in
-// registers (round to nearest) every 512 products, which costs one more read of it
-// for each. Loss and lse of 4096 x 151936 x 3584 against 64 bits: 2.9e-7 (a plain
-// fp32 form: 5.5e-7).
+// registers (round to nearest) after a run of products, which costs one more read of
+// it for each. Above 128 rows every 512: loss and lse of 4096 x 151936 x 3584 are 2.9e-7
+// from 64 bits (a plain fp32 form: 5.5e-7) in 3.27 ms; every 256 would leave 1.5e-7 and
+// take 3.51. Up to 128 rows, where the weight's bytes are waited for, every 256: the loss of
+// one row of d 896, median and largest of 60: 1.6e-7 and 3.4e-6 (plain 9.9e-8, 3.2e-6; every
+// 512 4.6e-7, 7.8e-6) in 55.6 us (every 512 55.3, every 128 58.8). Products of one sign are
+// the worst case: 3e-7 of a logit in bf16, 2.6e-6 in f16, whose products have more bits to
+// lose, and every 256 1e-7 and 1.1e-6.
 template <int CG_>
 struct ScoreOp : LogitTiles<CG_> {
     static constexpr bool PROMOTE = true;
-    __device__ int group() const { return 8; }
+    __device__ int group() const { return CG_ == 1 ? 4 : 8; }
     struct Acc {
         float v[2][32];
     };
