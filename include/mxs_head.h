@@ -47,7 +47,7 @@ extern "C" {
  *             state (it may hold NaN) reaches no output. Above 128 rows it is not
  *             read either and costs no products.
  *   d_loss, d_lse  rows floats; either may be NULL
- * Products are accumulated in fp32, rounded towards zero within runs of 256 (up to
+ * Products are accumulated in fp32, rounded towards zero within runs of 128 (up to
  * 128 rows) or 512 and to nearest between them; maxima and sums of the softmax are
  * fp32. Limits: vocab, rows, d_model < 2^31 - 1024; temperature > 0.
  */

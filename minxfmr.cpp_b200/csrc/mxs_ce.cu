@@ -233,7 +233,7 @@ template <int CG_>
 struct LogitTiles {
     static constexpr int CG = CG_;
     static constexpr int EPI = 16, SWAP = 0;
-    static constexpr bool F8 = false, PROMOTE = false;
+    static constexpr bool F8 = false, PROMOTE = false, ASIDE = false;
     __device__ int group() const { return INT32_MAX; }
     CUtensorMap mh, mw;
     int format;
@@ -299,21 +299,54 @@ struct LogitTiles {
 // registers (round to nearest) after a run of products, which costs one more read of
 // it for each. Above 128 rows every 512: loss and lse of 4096 x 151936 x 3584 are 2.9e-7
 // from 64 bits (a plain fp32 form: 5.5e-7) in 3.27 ms; every 256 would leave 1.5e-7 and
-// take 3.51. Up to 128 rows, where the weight's bytes are waited for, every 256: the loss of
-// one row of d 896, median and largest of 60: 1.6e-7 and 3.4e-6 (plain 9.9e-8, 3.2e-6; every
-// 512 4.6e-7, 7.8e-6) in 55.6 us (every 512 55.3, every 128 58.8). Products of one sign are
-// the worst case: 3e-7 of a logit in bf16, 2.6e-6 in f16, whose products have more bits to
-// lose, and every 256 1e-7 and 1.1e-6.
+// take 3.51. Up to 128 rows, where the weight's bytes are waited for, every 128, and the
+// targets' logits, whose products lean to one sign where a model has learnt something, are
+// plain fp32 dot products, a row a CTA, by a warp that has nothing else to do: the loss of one
+// row of d 896, median, 95th percentile and largest of 200: 1.3e-7, 1.0e-6 and 2.2e-6 (a plain
+// fp32 form: 6.8e-8, 8.9e-7, 1.9e-6) in 55.3 us; every 256 2.0e-7, 1.5e-6, 2.6e-6 in 53.4; every
+// 512 without the dot products 2.5e-7, 4.8e-6, 7.8e-6 in 53.4. Products of one sign lose 3e-7 of
+// a logit in bf16 and 2.6e-6 in f16, whose products have more bits to lose, in runs of 512, a
+// fifth of that and less in runs of 128.
 template <int CG_>
 struct ScoreOp : LogitTiles<CG_> {
-    static constexpr bool PROMOTE = true;
-    __device__ int group() const { return CG_ == 1 ? 4 : 8; }
+    static constexpr bool PROMOTE = true, ASIDE = CG_ == 1;
+    __device__ int group() const { return CG_ == 1 ? 2 : 8; }
     struct Acc {
         float v[2][32];
     };
     float2* part;    // [tile][rows]
     float* ytarget;  // [rows]: the target's logit times the temperature
+    const uint16_t *h, *w;  // ASIDE: the operands that the maps read
+    int64_t ldh, ldw;
+    int d;
 
+    __device__ __forceinline__ float2 pair(uint32_t x) const {
+        if (this->format == 0) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    }
+    __device__ void aside(const Ctx& x, int lane) const {
+        for (int r = x.unit; r < x.kept; r += x.units) {
+            const int v = this->target_of(r);
+            if (v < 0) continue;
+            const uint16_t *a = h + r * ldh, *b = w + v * ldw;  // rows start on 16-byte boundaries
+            float s = 0.0f, s2 = 0.0f;
+            for (int j = lane; j < d / 8; j += 32) {
+                const uint4 p = reinterpret_cast<const uint4*>(a)[j], q = reinterpret_cast<const uint4*>(b)[j];
+                const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = pair(pw[i]), g = pair(qw[i]);
+                    s = fmaf(f.x, g.x, s);
+                    s2 = fmaf(f.y, g.y, s2);
+                }
+            }
+            for (int k = d / 8 * 8 + lane; k < d; k += 32) s = fmaf(pair(a[k]).x, pair(b[k]).x, s);
+            s += s2;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (lane == 0) ytarget[r] = s;
+        }
+    }
     __device__ void begin(Acc& a, const Tile&, const Lane&, const Ctx&) const {
 #pragma unroll
         for (int i = 0; i < 64; ++i) a.v[i / 32][i % 32] = 0.0f;
@@ -350,7 +383,7 @@ struct ScoreOp : LogitTiles<CG_> {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     if (mxs::gemm::is_column(hit - c0, j)) {
-                        ytarget[r] = v[j];
+                        if (!ASIDE) ytarget[r] = v[j];
                         v[j] = -INFINITY;
                     }
             }
@@ -521,7 +554,7 @@ template <typename T>
 struct ProductOp {
     static constexpr int CG = 2;
     static constexpr int EPI = 16, SWAP = 0;
-    static constexpr bool F8 = false, PROMOTE = false;
+    static constexpr bool F8 = false, PROMOTE = false, ASIDE = false;
     // Sums of more than 32768 products are added up in fp32 after so many: the MMA's own
     // sum rounds towards zero at every 16 of them, which by then may have cost 2^-13 of it
     // (2 million rows of one sign, in one run: 8 parts in a thousand).
@@ -1055,7 +1088,13 @@ int score(const Call& a, const Plan& pl, const void* w, int64_t ldw, float* loss
     op.nt = pl.nt;
     op.part = pl.part;
     op.ytarget = pl.ytarget;
-    const int64_t units = CG == 1 ? ceil_div(a.vocab, pl.span) : ceil_div(a.rows, 256) * pl.nt;
+    op.h = static_cast<const uint16_t*>(pl.direct ? a.hidden : pl.packed);
+    op.ldh = pl.direct ? a.ldh : pl.ldk;
+    op.w = static_cast<const uint16_t*>(w);
+    op.ldw = ldw;
+    op.d = (int)a.d;
+    // CG 1: a CTA for each span of columns, and for each row's target
+    const int64_t units = CG == 1 ? std::max(ceil_div(a.vocab, pl.span), a.rows) : ceil_div(a.rows, 256) * pl.nt;
     MXS_TRY(mxs::gemm::launch(op, (int)std::min<int64_t>(a.sms / CG, units), a.st));
     const int* pos = pl.direct ? nullptr : pl.pos;
     if (a.rows <= 64)

@@ -277,7 +277,7 @@ template <int CG_, typename O, int RUNS>
 struct MatmulOp {
     static constexpr int CG = CG_;
     static constexpr int EPI = 8, SWAP = 0, STEP = 8 * EPI;  // columns from one run of a thread to its next
-    static constexpr bool F8 = true, PROMOTE = true;
+    static constexpr bool F8 = true, PROMOTE = true, ASIDE = false;
     __device__ int group() const { return 1; }
     struct Acc {
         float v[RUNS][32];
@@ -376,7 +376,7 @@ struct MatmulOp {
 template <typename O, int NP>
 struct DecodeOp {
     static constexpr int CG = 1, EPI = 8, SWAP = NP;
-    static constexpr bool F8 = true, PROMOTE = true;
+    static constexpr bool F8 = true, PROMOTE = true, ASIDE = false;
     __device__ int group() const { return 1; }
     struct Acc {
         float v[NP];

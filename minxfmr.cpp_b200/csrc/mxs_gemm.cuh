@@ -3,6 +3,7 @@
 //
 //   warp 0      loads operand tiles (TMA, 128-byte swizzle) into a ring of stages
 //   warp 1      issues tcgen05.mma (one thread), accumulators in TMEM
+//   warp 2      what an Op wants done beside it all, if anything
 //   warps 4..   (Op::EPI of them, 8 or 16) read accumulators back (tcgen05.ld) and do
 //               the Op's epilogue: EPI / 4 warps share the 32 rows that the hardware
 //               gives a warp's place, each taking every (EPI / 4)-th run of 32 columns
@@ -351,6 +352,7 @@ __device__ __forceinline__ bool gather(Lane& me, const Ctx& x) {  // all epilogu
 //   a_mn(t), b_mn(t)       operand majors of a tile
 //   bytes(t)               bytes this CTA loads per block
 //   load(t, kb, sa, sb, bar, ctx)
+//   ASIDE, aside(ctx, lane)                             whether warp 2 has something to do, and what
 //   zero(t, me, ctx)                                    the epilogue of a tile without blocks
 //   group()                blocks after which an accumulator is read back
 //   ahead(t, me, ctx), epilogue(t, tmem, me, ctx, it, kb)  !PROMOTE: kb, the first block of what the
@@ -458,9 +460,13 @@ __device__ __forceinline__ void run(const Op& op) {
                 const int group = op.group() < t.kn ? op.group() : t.kn;
                 int in = 0;  // block of its group
                 for (int kb = 0; kb < t.kn; ++kb) {
-                    // the operands first: they are there long before an accumulator comes free, and
-                    // a wait costs 100 clocks even where it has nothing to wait for
-                    ok = wait(&ring->full[s], ph, ring) && (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring));
+                    // What comes last is waited for last, since a wait costs 100 clocks even where it
+                    // has nothing to wait for: a pair's operands are there long before an accumulator
+                    // comes free, up to 128 rows' (CG 1) are what memory is read for.
+                    if (CG == 1)
+                        ok = (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring)) && wait(&ring->full[s], ph, ring);
+                    else
+                        ok = wait(&ring->full[s], ph, ring) && (in > 0 || wait(&ring->tempty[buf], tph ^ 1, ring));
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     fence_after();
                     const bool last = in + 1 == group || kb == t.kn - 1;
@@ -495,6 +501,8 @@ __device__ __forceinline__ void run(const Op& op) {
                 __syncwarp();
                 mbar_wait_bounded(&ring->drain, 0);
             }
+        } else if (Op::ASIDE && warp == 2) {
+            if constexpr (Op::ASIDE) op.aside(ctx, lane);
         }
     } else {
         if constexpr (Op::EPI == 16)
